@@ -58,6 +58,7 @@ extern "C" {
 #define TPTC_TYPE_Q4_K 12
 #define TPTC_TYPE_Q5_K 13
 #define TPTC_TYPE_Q6_K 14
+#define TPTC_TYPE_BF16 30          /* batched serving operators only */
 
 typedef struct tptc_ctx tptc_ctx;
 typedef struct tptc_matrix tptc_matrix;
@@ -331,6 +332,82 @@ TPTC_API int tptc_attn_decode_noalloc(const float* d_q, const float* d_kraw, voi
  * nonzero word also re-zeroes the whole static array.  *out_code is 0 when no call has run on
  * this device.  Allocates nothing. */
 TPTC_API int tptc_attn_decode_noalloc_status(void* stream, int* out_code);
+
+/* ------------------------------------------------ batched serving operators
+ * No counterpart in the reference, which serves one sequence at a time: many sequences of
+ * different lengths in one launch, over a KV cache that is allocated page by page and held in
+ * 8 bits.  Device pointers belong to the caller and to the current device; nothing is
+ * allocated, and every call may be captured into a CUDA graph (make one call outside a
+ * capture first: it sets up the kernels).  Element types are TPTC_TYPE_F32, _F16 or _BF16.
+ *
+ * Ragged batches are described by device arrays: d_cu[n_seq + 1] are the ascending row offsets
+ * of the sequences in the packed row arrays (d_cu[0] >= 0, d_cu[n_seq] <= the row count that
+ * the call is given; rows outside are neither read nor written), and a host bound on the
+ * longest sequence sizes the launch.  Indices that live on the device are checked there: a
+ * sequence whose offsets, positions or length are out of range is left out, and a page id
+ * outside the cache is not followed; either sets *status to TPTC_ERR_ARG. */
+
+/* A paged KV cache in 8 bits: page p holds `page` consecutive positions of one sequence, for
+ * every kv head; code c of page p and head h stands for c * scale[p][h]. */
+typedef struct {
+    int8_t* k;             /* [n_pages][n_kv][page][head_dim] codes in -127..127, 16-byte aligned */
+    int8_t* v;             /* the same for V */
+    float* k_scale;        /* [n_pages][n_kv] */
+    float* v_scale;
+    const int32_t* table;  /* [n_seq][max_pages] page ids: position i of sequence b lies in page
+                              table[b][i / page], row i % page */
+    int32_t* status;       /* device word, zero at first: receives TPTC_ERR_* (see above); may be NULL */
+    int32_t n_pages, page; /* page: 16, 32 or 64 positions */
+    int32_t n_kv, head_dim; /* head_dim 64, 96 or 128 */
+    int32_t n_seq, max_pages;
+} tptc_kv8;
+
+/* Rotary positions: f32 tables [rows][dim / 2] of cos and sin by position (any base or length
+ * scaling is in the tables), over the first `dim` elements of a head (a multiple of 16, at most
+ * head_dim; the rest pass unrotated).  halves 0: pairs (2i, 2i + 1), as tptc_attn_decode;
+ * 1: pairs (i, i + dim / 2). */
+typedef struct {
+    const float* cos;      /* 16-byte aligned */
+    const float* sin;
+    int32_t rows, dim, halves;
+} tptc_rope;
+
+/* Appends new keys and values to the cache, rotated on the way; the same pass rotates the queries.
+ * Packed row t of sequence b (d_cu[b] <= t < d_cu[b + 1]) is position d_start[b] + t - d_cu[b].
+ *   d_q / d_k / d_v: rows of `type`, row t at element t * q_stride (k_stride, v_stride), heads
+ *     adjacent (n_heads x head_dim, n_kv x head_dim): slices of a fused projection fit.  16-byte
+ *     aligned, strides multiples of 16 bytes.  d_q and n_heads may be NULL and 0.
+ *   d_q_out, d_k_out: the rotated rows, contiguous, of `type`; each may be NULL (not wanted).
+ *     d_q_out may be d_q itself, and d_k_out d_k, where the stride leaves no gap.
+ *   rope: NULL stores and copies without rotating.
+ * One scale per (page, kv head): with a the largest magnitude of the new rows in the page,
+ * s = max(s_old, a * (1/127)), where s_old counts only if earlier positions of the sequence lie in the
+ * page; a new code is x / s rounded to nearest even, and where s grows the earlier codes c become c * s_old / s,
+ * rounded.  A scale below the smallest normal float is 0.  A page that receives a value that is
+ * not finite gets scale NaN, so whatever attends to it becomes NaN.  Rows of the page behind
+ * the last new position keep their codes.  No two sequences of one call may append to the same page.
+ * max_new: no sequence brings more new rows (n_tokens in all). */
+TPTC_API int tptc_kv8_append(const tptc_kv8* cache, const tptc_rope* rope, int type, const void* d_q,
+                             int64_t q_stride, const void* d_k, int64_t k_stride, const void* d_v,
+                             int64_t v_stride, int n_heads, void* d_q_out, void* d_k_out, const int32_t* d_cu,
+                             const int32_t* d_start, int n_tokens, int max_new, void* stream);
+
+/* The values that positions d_start[b] .. of each sequence stand for, as packed rows [n_tokens][n_kv][head_dim]
+ * of `type` (code * scale in f32, rounded once): the K and V that tptc_attn_packed takes to
+ * continue a cached prefix.  Either output may be NULL. */
+TPTC_API int tptc_kv8_read(const tptc_kv8* cache, int type, const int32_t* d_cu, const int32_t* d_start,
+                           int n_tokens, int max_rows, void* d_k_out, void* d_v_out, void* stream);
+
+/* Log probabilities of given tokens beside tptc_sample, in one pass over the logits: rows of `vocab` logits of
+ * `type`, row r at element r * row_stride (any alignment of whole elements).
+ *   d_logprob[r] = log softmax(row)[d_token[r]] (both NULL: not wanted; an id outside the
+ *     vocabulary gives NaN); d_entropy[r] (nats, may be NULL);
+ *   d_top_id, d_top_logprob [rows][n_top]: the n_top <= 32 largest, in descending order, equal logits
+ *     by ascending id (n_top 0: not wanted; NaN logits count as largest).  n_top <= vocab.
+ * Sums are f32.  -inf logits have probability 0; a NaN or +inf logit, or a row of -inf alone, gives NaN. */
+TPTC_API int tptc_logprobs(int type, const void* d_logits, int rows, int vocab, int64_t row_stride,
+                           const int32_t* d_token, float* d_logprob, float* d_entropy, int n_top, int32_t* d_top_id,
+                           float* d_top_logprob, void* stream);
 
 #ifdef __cplusplus
 }

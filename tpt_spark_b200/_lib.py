@@ -32,6 +32,16 @@ class InferParamsC(ctypes.Structure):
                 ("seed", c_u64), ("eos_token_id", c_i64)]
 
 
+class Kv8C(ctypes.Structure):
+    _fields_ = [("k", c_vp), ("v", c_vp), ("k_scale", c_vp), ("v_scale", c_vp), ("table", c_vp), ("status", c_vp),
+                ("n_pages", c_int), ("page", c_int), ("n_kv", c_int), ("head_dim", c_int), ("n_seq", c_int),
+                ("max_pages", c_int)]
+
+
+class RopeC(ctypes.Structure):
+    _fields_ = [("cos", c_vp), ("sin", c_vp), ("rows", c_int), ("dim", c_int), ("halves", c_int)]
+
+
 TOKEN_CB = ctypes.CFUNCTYPE(c_int, c_u32, c_int, c_vp)
 PROGRESS_CB = ctypes.CFUNCTYPE(None, c_u32, c_u32, c_vp)
 
@@ -85,6 +95,10 @@ SIGNATURES = {
     "tptc_attn_decode_noalloc": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int,
                                          c_vp, c_vp]),
     "tptc_attn_decode_noalloc_status": (c_int, [c_vp, ctypes.POINTER(c_int)]),
+    "tptc_kv8_append": (c_int, [c_vp, c_vp, c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_int, c_vp, c_vp, c_vp, c_vp,
+                                c_int, c_int, c_vp]),
+    "tptc_kv8_read": (c_int, [c_vp, c_int, c_vp, c_vp, c_int, c_int, c_vp, c_vp, c_vp]),
+    "tptc_logprobs": (c_int, [c_int, c_vp, c_int, c_int, c_i64, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp]),
 }
 
 _L = None

@@ -11,6 +11,7 @@
 #include "engine.h"
 #include "kernels.h"
 #include "prefill.h"
+#include "serve.h"
 #include "tp.h"
 #include "tptc.h"
 
@@ -593,6 +594,123 @@ TPTC_API int tptc_block_dots(const tptc_matrix* m, const float* d_x, int32_t* d_
     p.msum = d_msum;
     cudaError_t e = tptc::gemv_launch(p, tptc::EPI_DOTS, static_cast<cudaStream_t>(stream), false);
     return e == cudaSuccess ? TPTC_OK : cuda_fail(e, "block_dots");
+}
+
+// ---- batched serving operators
+
+static bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
+static int kv8_args(const tptc_kv8* c, int type) {
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || !c->table)
+        return fail_code(nullptr, TPTC_ERR_ARG, "kv8: null cache pointer");
+    if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128)
+        return fail_code(nullptr, TPTC_ERR_UNSUPPORTED, "kv8: head_dim must be 64, 96 or 128");
+    if (c->page != 16 && c->page != 32 && c->page != 64)
+        return fail_code(nullptr, TPTC_ERR_UNSUPPORTED, "kv8: page must be 16, 32 or 64 positions");
+    if (type != TPTC_TYPE_F32 && type != TPTC_TYPE_F16 && type != TPTC_TYPE_BF16)
+        return fail_code(nullptr, TPTC_ERR_UNSUPPORTED, "kv8: type must be TPTC_TYPE_F32, _F16 or _BF16");
+    if (c->n_pages <= 0 || c->n_kv <= 0 || c->n_seq < 0 || c->max_pages <= 0)
+        return fail_code(nullptr, TPTC_ERR_ARG, "kv8: bad cache sizes");
+    if ((int64_t)c->max_pages * c->page > INT32_MAX)
+        return fail_code(nullptr, TPTC_ERR_ARG, "kv8: a sequence's positions must fit 31 bits");
+    if (misaligned(c->k, 16) || misaligned(c->v, 16))
+        return fail_code(nullptr, TPTC_ERR_ARG, "kv8: k and v must be 16-byte aligned");
+    return TPTC_OK;
+}
+
+// Rows of `type` at a stride: 16-byte aligned, each row holding `width` elements.
+static bool bad_rows(const void* p, int64_t stride, int64_t width, int type) {
+    const int e = type == TPTC_TYPE_F32 ? 4 : 2;
+    return misaligned(p, 16) || stride < width || stride % (16 / e) != 0;
+}
+
+TPTC_API int tptc_kv8_append(const tptc_kv8* cache, const tptc_rope* rope, int type, const void* d_q,
+                             int64_t q_stride, const void* d_k, int64_t k_stride, const void* d_v, int64_t v_stride,
+                             int n_heads, void* d_q_out, void* d_k_out, const int32_t* d_cu, const int32_t* d_start,
+                             int n_tokens, int max_new, void* stream) {
+    if (int rc = kv8_args(cache, type)) return rc;
+    if (n_tokens < 0 || max_new < 0) return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: negative row count");
+    if (!d_k || !d_v || !d_cu || !d_start) return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: null pointer");
+    const int hd = cache->head_dim;
+    if (bad_rows(d_k, k_stride, (int64_t)cache->n_kv * hd, type) || bad_rows(d_v, v_stride, (int64_t)cache->n_kv * hd, type) ||
+        misaligned(d_k_out, 16))
+        return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: k and v rows must be 16-byte aligned and not overlap");
+    if (d_q_out) {
+        if (!d_q || n_heads <= 0 || n_heads % cache->n_kv)
+            return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: n_heads must be a positive multiple of n_kv");
+        if (bad_rows(d_q, q_stride, (int64_t)n_heads * hd, type) || misaligned(d_q_out, 16))
+            return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: q rows must be 16-byte aligned and not overlap");
+    }
+    if (rope && (!rope->cos || !rope->sin || misaligned(rope->cos, 16) || misaligned(rope->sin, 16) || rope->rows <= 0 ||
+                 rope->dim <= 0 || rope->dim % 16 || rope->dim > hd))
+        return fail_code(nullptr, TPTC_ERR_ARG,
+                         "kv8_append: rope tables must be 16-byte aligned, dim a multiple of 16 up to head_dim");
+    if (n_tokens == 0 || max_new == 0 || cache->n_seq == 0) return TPTC_OK;
+    tptc::Kv8Append p = {};
+    p.c = *cache;
+    if (rope) p.rope = *rope;
+    p.q = d_q;
+    p.k = d_k;
+    p.v = d_v;
+    p.q_stride = q_stride;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.n_heads = n_heads;
+    p.q_out = d_q_out;
+    p.k_out = d_k_out;
+    p.cu = d_cu;
+    p.start = d_start;
+    p.n_tokens = n_tokens;
+    p.max_new = max_new;
+    cudaError_t e = tptc::launch_kv8_append(type, p, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? TPTC_OK : cuda_fail(e, "kv8_append");
+}
+
+TPTC_API int tptc_kv8_read(const tptc_kv8* cache, int type, const int32_t* d_cu, const int32_t* d_start, int n_tokens,
+                           int max_rows, void* d_k_out, void* d_v_out, void* stream) {
+    if (int rc = kv8_args(cache, type)) return rc;
+    if (n_tokens < 0 || max_rows < 0) return fail_code(nullptr, TPTC_ERR_ARG, "kv8_read: negative row count");
+    if (!d_cu || !d_start || misaligned(d_k_out, 16) || misaligned(d_v_out, 16))
+        return fail_code(nullptr, TPTC_ERR_ARG, "kv8_read: null offsets or misaligned output");
+    if (n_tokens == 0 || max_rows == 0 || cache->n_seq == 0 || (!d_k_out && !d_v_out)) return TPTC_OK;
+    tptc::Kv8Read p = {};
+    p.c = *cache;
+    p.cu = d_cu;
+    p.start = d_start;
+    p.n_tokens = n_tokens;
+    p.max_rows = max_rows;
+    p.k_out = d_k_out;
+    p.v_out = d_v_out;
+    cudaError_t e = tptc::launch_kv8_read(type, p, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? TPTC_OK : cuda_fail(e, "kv8_read");
+}
+
+TPTC_API int tptc_logprobs(int type, const void* d_logits, int rows, int vocab, int64_t row_stride,
+                           const int32_t* d_token, float* d_logprob, float* d_entropy, int n_top, int32_t* d_top_id,
+                           float* d_top_logprob, void* stream) {
+    if (type != TPTC_TYPE_F32 && type != TPTC_TYPE_F16 && type != TPTC_TYPE_BF16)
+        return fail_code(nullptr, TPTC_ERR_UNSUPPORTED, "logprobs: type must be TPTC_TYPE_F32, _F16 or _BF16");
+    if (!d_logits || rows < 0 || vocab <= 0 || row_stride < vocab || misaligned(d_logits, type == TPTC_TYPE_F32 ? 4 : 2))
+        return fail_code(nullptr, TPTC_ERR_ARG, "logprobs: bad logits");
+    if (!d_token != !d_logprob) return fail_code(nullptr, TPTC_ERR_ARG, "logprobs: d_token and d_logprob go together");
+    if (n_top < 0 || n_top > tptc::kMaxTop || n_top > vocab || (n_top > 0 && (!d_top_id || !d_top_logprob)))
+        return fail_code(nullptr, TPTC_ERR_ARG, "logprobs: n_top must be 0 .. min(32, vocab), with both outputs");
+    if (rows == 0) return TPTC_OK;
+    int dev = 0, sms = 0;
+    if (int rc = ensure_kernels(&dev, &sms)) return rc;
+    tptc::LogprobParams p = {};
+    p.logits = d_logits;
+    p.rows = rows;
+    p.vocab = vocab;
+    p.row_stride = row_stride;
+    p.token = d_token;
+    p.logprob = d_logprob;
+    p.entropy = d_entropy;
+    p.n_top = n_top;
+    p.top_id = d_top_id;
+    p.top_logprob = d_top_logprob;
+    cudaError_t e = tptc::launch_logprobs(type, p, sms, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? TPTC_OK : cuda_fail(e, "logprobs");
 }
 
 }  // extern "C"

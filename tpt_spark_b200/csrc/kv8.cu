@@ -1,0 +1,339 @@
+// kv8.cu -- the paged 8-bit KV cache: appending a ragged batch of new keys and values (with the
+// position rotation of q and k in the same pass) and reading positions back as dense rows.
+//
+// Append.  A page of one kv head has one scale s, and its codes are c = rint(x / s), |c| <= 127.
+// With a = max |x| over the page's new rows, s' = max(s, a / 127); where s' > s the earlier codes
+// become rint(c s / s'), so a value moves by at most half a step s' each time the scale grows.
+// The maximum over the page couples all of its new rows, hence the split: one CTA per (sequence,
+// touched page, kv head), which keeps the page's rotated rows in registers between the maximum
+// and the rounding (each input is read once) and rotates the query rows of its head group and
+// positions, so one launch moves q, k and v.  Bound by HBM for prompts and by launch latency for
+// decode steps.
+#include <algorithm>
+
+#include "serve.h"
+
+namespace tptc {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ void flag(int32_t* status) {
+    if (status) atomicExch(status, TPTC_ERR_ARG);
+}
+
+// Rows [r0, r1) of sequence b lie in page `p` of its table; false when there are none.
+struct Span {
+    int first, n;   // packed row of the first, and how many
+    int off;        // their first row in the page
+    int pos;        // position of the first
+    int page_id;    // -1: not in the cache
+};
+__device__ __forceinline__ bool page_span(const tptc_kv8& c, const int32_t* cu, const int32_t* start, int n_rows,
+                                          int most, int rope_rows, int b, int u, Span& s) {
+    const int lo = cu[b], hi = cu[b + 1], begin = start[b];
+    if (lo == hi) return false;
+    const int64_t cap = (int64_t)c.max_pages * c.page, end = (int64_t)begin + hi - lo;
+    if (lo < 0 || hi < lo || hi > n_rows || hi - lo > most || begin < 0 || end > cap || (rope_rows >= 0 && end > rope_rows)) {
+        if (u == 0 && threadIdx.x == 0) flag(c.status);
+        return false;
+    }
+    const int64_t p = begin / c.page + u, r0 = max((int64_t)begin, p * c.page), r1 = min(end, (p + 1) * c.page);
+    if (r0 >= r1) return false;
+    s.first = lo + (int)(r0 - begin);
+    s.n = (int)(r1 - r0);
+    s.off = (int)(r0 - p * c.page);
+    s.pos = (int)r0;
+    const int id = c.table[(int64_t)b * c.max_pages + p];
+    s.page_id = id >= 0 && id < c.n_pages ? id : -1;
+    if (s.page_id < 0 && threadIdx.x == 0) flag(c.status);
+    return true;
+}
+
+// Rotates elements [8 lg, 8 lg + 8) of a row held by a group of lanes (lane lg of the group holds
+// those elements).  Each product and sum is rounded by itself, as the framework's other
+// rotations do.  Every lane of the warp takes part (the halves form exchanges vectors).
+template <typename T>
+__device__ __forceinline__ void rotate8(float (&x)[8], int lg, int pos, bool valid, const tptc_rope& r) {
+    const int c = 8 * lg;
+    const bool in = valid && c < r.dim;
+    if (!r.halves) {
+        if (!in) return;
+        const int64_t at = (int64_t)pos * (r.dim / 2) + c / 2;
+        const float4 cs = __ldg(reinterpret_cast<const float4*>(r.cos + at));
+        const float4 sn = __ldg(reinterpret_cast<const float4*>(r.sin + at));
+        const float cc[4] = {cs.x, cs.y, cs.z, cs.w}, ss[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float a = x[2 * i], b = x[2 * i + 1];
+            x[2 * i] = __fsub_rn(__fmul_rn(a, cc[i]), __fmul_rn(b, ss[i]));
+            x[2 * i + 1] = __fadd_rn(__fmul_rn(a, ss[i]), __fmul_rn(b, cc[i]));
+        }
+        return;
+    }
+    const int half = r.dim / 2, delta = half / 8;
+    const bool second = c >= half;
+    const int lane = threadIdx.x & 31, src = in ? (second ? lane - delta : lane + delta) : lane;
+    float y[8];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = __shfl_sync(0xffffffffu, x[i], src);
+    } else {  // the values are T exactly: exchange them in pairs
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t w = __shfl_sync(0xffffffffu, pack2<T>(x[2 * i], x[2 * i + 1]), src);
+            const T* h = reinterpret_cast<const T*>(&w);
+            y[2 * i] = to_f32(h[0]), y[2 * i + 1] = to_f32(h[1]);
+        }
+    }
+    if (!in) return;
+    const int64_t at = (int64_t)pos * half + (second ? c - half : c);
+    float cc[8], ss[8];
+    load8(r.cos + at, cc);
+    load8(r.sin + at, ss);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float xc = __fmul_rn(x[i], cc[i]), ys = __fmul_rn(y[i], ss[i]);
+        x[i] = second ? __fadd_rn(ys, xc) : __fsub_rn(xc, ys);
+    }
+}
+
+// Scale of a page after values of magnitude up to `top` joined it (inf or NaN: not finite).
+__device__ __forceinline__ float grown_scale(float old, float top) {
+    if (!(top <= 3.402823466e38f) || isnan(old)) return __int_as_float(0x7fc00000);
+    const float s = fmaxf(old, __fmul_rn(top, 1.f / 127.f));
+    return s < 1.17549435e-38f ? 0.f : s;
+}
+
+__device__ __forceinline__ int code_of(float x, float inv) {
+    // a NaN (only where the scale is NaN) converts to 0
+    return max(-127, min(127, __float2int_rn(__fmul_rn(x, inv))));
+}
+
+__device__ __forceinline__ void store_codes(int8_t* dst, const float (&x)[8], float inv) {
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        w[h] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[h] |= (uint32_t)(code_of(x[4 * h + i], inv) & 255) << (8 * i);
+    }
+    *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+}
+
+// The earlier codes of the page (n of them, a multiple of 16) after the scale grew.
+__device__ __forceinline__ void rescale_codes(int8_t* codes, int n, float ratio) {
+    for (int i = threadIdx.x; i < n / 16; i += kThreads) {
+        uint4* at = reinterpret_cast<uint4*>(codes) + i;
+        uint4 w = *at;
+        uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            uint32_t o = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int c = (int8_t)(r[k] >> (8 * j));
+                o |= (uint32_t)(__float2int_rn(__fmul_rn((float)c, ratio)) & 255) << (8 * j);
+            }
+            r[k] = o;
+        }
+        *at = make_uint4(r[0], r[1], r[2], r[3]);
+    }
+}
+
+// NR: passes of the CTA over a page's rows (16 or 32 rows each).
+template <typename T, int HD, int NR>
+__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_constant__ Kv8Append p) {
+    constexpr int GS = HD == 64 ? 8 : 16;  // lanes per row (12 of 16 work at head_dim 96)
+    constexpr int RP = kThreads / GS;
+    __shared__ float s_top[2][kThreads / 32];
+    const int tid = threadIdx.x, lg = tid % GS, grp = tid / GS, c = 8 * lg;
+    const bool lane_in = c < HD;
+    const int h = blockIdx.x % p.c.n_kv, unit = blockIdx.x / p.c.n_kv, u = unit % p.units, b = unit / p.units;
+    Span s;
+    if (!page_span(p.c, p.cu, p.start, p.n_tokens, p.max_new, p.rope.dim ? p.rope.rows : -1, b, u, s)) return;
+
+    const T* kin = static_cast<const T*>(p.k) + (int64_t)s.first * p.k_stride + h * HD + c;
+    const T* vin = static_cast<const T*>(p.v) + (int64_t)s.first * p.v_stride + h * HD + c;
+    float xk[NR][8], xv[NR][8];
+    float top_k = 0.f, top_v = 0.f;
+    bool odd_k = false, odd_v = false;  // a value that is not finite
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const int row = grp + i * RP;
+        const bool in = lane_in && row < s.n;
+#pragma unroll
+        for (int e = 0; e < 8; e++) xk[i][e] = xv[i][e] = 0.f;
+        if (in) {
+            load8(kin + row * p.k_stride, xk[i]);
+            load8(vin + row * p.v_stride, xv[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const int row = grp + i * RP;
+        const bool in = lane_in && row < s.n;
+        if (p.rope.dim) rotate8<T>(xk[i], lg, s.pos + row, in, p.rope);
+        if (in && p.k_out)
+            store8(static_cast<T*>(p.k_out) + ((int64_t)(s.first + row) * p.c.n_kv + h) * HD + c, xk[i]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float a = fabsf(xk[i][e]), d = fabsf(xv[i][e]);
+            odd_k |= !(a <= 3.402823466e38f);
+            odd_v |= !(d <= 3.402823466e38f);
+            top_k = fmaxf(top_k, a);
+            top_v = fmaxf(top_v, d);
+        }
+    }
+    if (odd_k) top_k = INFINITY;
+    if (odd_v) top_v = INFINITY;
+    top_k = warp_max(top_k);
+    top_v = warp_max(top_v);
+    if ((tid & 31) == 0) s_top[0][tid >> 5] = top_k, s_top[1][tid >> 5] = top_v;
+
+    const int64_t at = (int64_t)s.page_id * p.c.n_kv + h;
+    const bool store = s.page_id >= 0;
+    float old_k = 0.f, old_v = 0.f;
+    if (store && s.off > 0) old_k = p.c.k_scale[at], old_v = p.c.v_scale[at];
+
+    if (p.q_out) {  // the queries of this head group at the same positions
+        const int G = p.n_heads / p.c.n_kv, rows = s.n * G;
+        const T* qin = static_cast<const T*>(p.q) + (int64_t)s.first * p.q_stride + (int64_t)h * G * HD + c;
+        T* qout = static_cast<T*>(p.q_out) + ((int64_t)s.first * p.n_heads + (int64_t)h * G) * HD + c;
+        for (int r0 = 0; r0 < rows; r0 += RP) {
+            const int r = r0 + grp, t = r / G, g = r - t * G;
+            const bool in = lane_in && r < rows;
+            float x[8] = {};
+            if (in) load8(qin + (int64_t)t * p.q_stride + g * HD, x);
+            if (p.rope.dim) rotate8<T>(x, lg, s.pos + t, in, p.rope);
+            if (in) store8(qout + ((int64_t)t * p.n_heads + g) * HD, x);
+        }
+    }
+    __syncthreads();  // the maxima are in; every thread has read the old scales
+    if (!store) return;
+    top_k = s_top[0][0], top_v = s_top[1][0];
+#pragma unroll
+    for (int w = 1; w < kThreads / 32; w++) top_k = fmaxf(top_k, s_top[0][w]), top_v = fmaxf(top_v, s_top[1][w]);
+    const float new_k = grown_scale(old_k, top_k), new_v = grown_scale(old_v, top_v);
+    int8_t* ck = p.c.k + at * p.c.page * HD;
+    int8_t* cv = p.c.v + at * p.c.page * HD;
+    const float inv_k = new_k > 0.f ? __frcp_rn(new_k) : 0.f, inv_v = new_v > 0.f ? __frcp_rn(new_v) : 0.f;
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const int row = grp + i * RP;
+        if (!lane_in || row >= s.n) continue;
+        store_codes(ck + (s.off + row) * HD + c, xk[i], inv_k);
+        store_codes(cv + (s.off + row) * HD + c, xv[i], inv_v);
+    }
+    if (s.off > 0) {  // (a scale that is NaN compares false: the codes stay)
+        if (new_k > old_k) rescale_codes(ck, s.off * HD, __fdiv_rn(old_k, new_k));
+        if (new_v > old_v) rescale_codes(cv, s.off * HD, __fdiv_rn(old_v, new_v));
+    }
+    if (tid == 0) p.c.k_scale[at] = new_k, p.c.v_scale[at] = new_v;
+}
+
+// Sixteen codes as values: byte b of a word, offset to 0..255, in the mantissa of 2^23 + b, is exact.
+template <typename T>
+__device__ __forceinline__ void store_values(T* dst, const uint4& w, float scale) {
+    const uint32_t r[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+    float x[2][8];
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float f = __uint_as_float(__byte_perm(r[k], 0x4b000000u, 0x7440 + j)) - 8388736.f;
+            x[k >> 1][(k & 1) * 4 + j] = __fmul_rn(f, scale);
+        }
+    store8(dst, x[0]);
+    store8(dst + 8, x[1]);
+}
+
+// One CTA per (sequence, page, group of kv heads): 16 codes per thread and load, a page's rows of
+// one head contiguous, so that loads and stores both run along head_dim.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constant__ Kv8Read p) {
+    constexpr int CH = HD / 16;
+    const int groups = (p.c.n_kv + p.heads_per_cta - 1) / p.heads_per_cta;
+    const int g = blockIdx.x % groups, unit = blockIdx.x / groups, u = unit % p.units, b = unit / p.units;
+    Span s;
+    if (!page_span(p.c, p.cu, p.start, p.n_tokens, p.max_rows, -1, b, u, s) || s.page_id < 0) return;
+    const int h0 = g * p.heads_per_cta, heads = min(p.heads_per_cta, p.c.n_kv - h0);
+    const int per = s.n * CH, total = heads * per;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+        const int hh = i / per, rem = i - hh * per, row = rem / CH, ch = rem - row * CH;
+        const int64_t at = (int64_t)s.page_id * p.c.n_kv + h0 + hh;
+        const int64_t src = (at * p.c.page + s.off + row) * HD + ch * 16;
+        const int64_t dst = ((int64_t)(s.first + row) * p.c.n_kv + h0 + hh) * HD + ch * 16;
+        if (p.k_out) {
+            const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p.c.k + src));
+            store_values(static_cast<T*>(p.k_out) + dst, w, p.c.k_scale[at]);
+        }
+        if (p.v_out) {
+            const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p.c.v + src));
+            store_values(static_cast<T*>(p.v_out) + dst, w, p.c.v_scale[at]);
+        }
+    }
+}
+
+template <typename P>
+cudaError_t launch(void (*kernel)(P), int64_t ctas, const P& p, cudaStream_t st) {
+    if (ctas <= 0 || ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <typename T, int HD>
+cudaError_t append_hd(const Kv8Append& p, int64_t ctas, cudaStream_t st) {
+    constexpr int RP = kThreads / (HD == 64 ? 8 : 16);
+    const int passes = (p.c.page + RP - 1) / RP;
+    if (passes <= 1) return launch(kv8_append_kernel<T, HD, 1>, ctas, p, st);
+    if (passes == 2) return launch(kv8_append_kernel<T, HD, 2>, ctas, p, st);
+    if constexpr (HD != 64) return launch(kv8_append_kernel<T, HD, 4>, ctas, p, st);
+    return cudaErrorInvalidValue;
+}
+
+template <typename T>
+cudaError_t append_t(const Kv8Append& p, int64_t ctas, cudaStream_t st) {
+    if (p.c.head_dim == 64) return append_hd<T, 64>(p, ctas, st);
+    if (p.c.head_dim == 96) return append_hd<T, 96>(p, ctas, st);
+    return append_hd<T, 128>(p, ctas, st);
+}
+
+template <typename T>
+cudaError_t read_t(const Kv8Read& p, int64_t ctas, cudaStream_t st) {
+    if (p.c.head_dim == 64) return launch(kv8_read_kernel<T, 64>, ctas, p, st);
+    if (p.c.head_dim == 96) return launch(kv8_read_kernel<T, 96>, ctas, p, st);
+    return launch(kv8_read_kernel<T, 128>, ctas, p, st);
+}
+
+// Pages that n consecutive positions can touch, wherever they begin.
+int touched_pages(int n, int page) { return (int)(((int64_t)n + page - 2) / page + 1); }
+
+}  // namespace
+
+cudaError_t launch_kv8_append(int type, Kv8Append p, cudaStream_t st) {
+    p.units = touched_pages(std::min(p.max_new, p.n_tokens), p.c.page);
+    const int64_t ctas = (int64_t)p.c.n_seq * p.units * p.c.n_kv;
+    if (type == TPTC_TYPE_F16) return append_t<__half>(p, ctas, st);
+    if (type == TPTC_TYPE_BF16) return append_t<__nv_bfloat16>(p, ctas, st);
+    return append_t<float>(p, ctas, st);
+}
+
+cudaError_t launch_kv8_read(int type, Kv8Read p, cudaStream_t st) {
+    p.units = touched_pages(std::min(p.max_rows, p.n_tokens), p.c.page);
+    // about 16 KB of codes per CTA and tensor
+    p.heads_per_cta = std::max(1, std::min(p.c.n_kv, 16384 / (p.c.page * p.c.head_dim)));
+    const int64_t ctas = (int64_t)p.c.n_seq * p.units * ceil_div(p.c.n_kv, p.heads_per_cta);
+    if (type == TPTC_TYPE_F16) return read_t<__half>(p, ctas, st);
+    if (type == TPTC_TYPE_BF16) return read_t<__nv_bfloat16>(p, ctas, st);
+    return read_t<float>(p, ctas, st);
+}
+
+cudaError_t serve_init_device() { return logprobs_init_device(); }
+
+}  // namespace tptc

@@ -9,6 +9,7 @@ namespace tptc {
 
 cudaError_t attn_init_device();
 cudaError_t prefill_init_device();
+cudaError_t serve_init_device();
 
 namespace {
 
@@ -214,7 +215,9 @@ cudaError_t kernels_init_device() {
     if (e != cudaSuccess) return e;
     e = attn_init_device();
     if (e != cudaSuccess) return e;
-    return prefill_init_device();
+    e = prefill_init_device();
+    if (e != cudaSuccess) return e;
+    return serve_init_device();
 }
 
 }  // namespace tptc

@@ -10,14 +10,18 @@ from typing import Optional
 
 import numpy as np
 
-from ._lib import check, lib
+from ._lib import Kv8C, RopeC, check, lib
 
-F32, F16, Q8_0, Q4_K, Q6_K = 0, 1, 8, 12, 14
+F32, F16, Q8_0, Q4_K, Q6_K, BF16 = 0, 1, 8, 12, 14, 30
 Q4_0, Q4_1, Q5_0, Q5_1, Q2_K, Q3_K, Q5_K = 2, 3, 6, 7, 10, 11, 13
 
 
 def _ptr(t) -> int:
     return t if isinstance(t, int) else t.data_ptr()
+
+
+def _opt(t) -> Optional[int]:
+    return None if t is None else _ptr(t)
 
 
 def dequant(ggml_type: int, d_blocks, n: int, d_out, stream: Optional[int] = None) -> None:
@@ -120,3 +124,47 @@ def attn_prefill(d_q, d_kcache, d_vcache, d_out, T: int, start: int, n_heads: in
     """Causal GQA attention of T prompt rows at positions start.. over an fp16 KV cache."""
     check(lib().tptc_attn_prefill(_ptr(d_q), _ptr(d_kcache), _ptr(d_vcache), _ptr(d_out), T, start, n_heads, n_kv,
                                   head_dim, max_seq, stream))
+
+
+class Rope:
+    """Rotary tables (tptc_rope): f32 cos / sin [rows][dim / 2] by position over the first `dim`
+    elements of a head; halves: pairs (i, i + dim / 2) instead of (2i, 2i + 1)."""
+
+    def __init__(self, d_cos, d_sin, rows: int, dim: int, halves: bool = False):
+        self._keep = (d_cos, d_sin)
+        self._c = RopeC(_ptr(d_cos), _ptr(d_sin), rows, dim, int(halves))
+        self._h = ctypes.addressof(self._c)
+
+
+class Kv8Cache:
+    """A paged 8-bit KV cache (tptc_kv8) over the caller's device buffers: codes [n_pages][n_kv][page][head_dim],
+    scales [n_pages][n_kv], page table [n_seq][max_pages] (int32) and an int32 status word that is zero
+    at first and receives an error code when an index on the device is out of range."""
+
+    def __init__(self, d_k, d_v, d_k_scale, d_v_scale, d_table, d_status, n_pages: int, page: int, n_kv: int,
+                 head_dim: int, n_seq: int, max_pages: int):
+        self._keep = (d_k, d_v, d_k_scale, d_v_scale, d_table, d_status)
+        self._c = Kv8C(_ptr(d_k), _ptr(d_v), _ptr(d_k_scale), _ptr(d_v_scale), _ptr(d_table), _opt(d_status), n_pages,
+                       page, n_kv, head_dim, n_seq, max_pages)
+        self._h = ctypes.addressof(self._c)
+
+    def append(self, rope: Optional[Rope], type_: int, d_q, q_stride: int, d_k, k_stride: int, d_v, v_stride: int,
+               n_heads: int, d_q_out, d_k_out, d_cu, d_start, n_tokens: int, max_new: int,
+               stream: Optional[int] = None) -> None:
+        """New keys and values of a ragged batch into the cache, rotated on the way with q (tptc_kv8_append)."""
+        check(lib().tptc_kv8_append(self._h, None if rope is None else rope._h, type_, _opt(d_q), q_stride, _ptr(d_k),
+                                    k_stride, _ptr(d_v), v_stride, n_heads, _opt(d_q_out), _opt(d_k_out), _ptr(d_cu),
+                                    _ptr(d_start), n_tokens, max_new, stream))
+
+    def read(self, d_cu, d_start, n_tokens: int, max_rows: int, type_: int, d_k_out, d_v_out,
+             stream: Optional[int] = None) -> None:
+        """The values of ranges of positions as packed dense rows (tptc_kv8_read)."""
+        check(lib().tptc_kv8_read(self._h, type_, _ptr(d_cu), _ptr(d_start), n_tokens, max_rows, _opt(d_k_out),
+                                  _opt(d_v_out), stream))
+
+
+def logprobs(d_logits, type_: int, rows: int, vocab: int, row_stride: int, d_token, d_logprob, d_entropy, n_top: int,
+             d_top_id, d_top_logprob, stream: Optional[int] = None) -> None:
+    """Log probabilities of given tokens, entropy and the n_top largest of each row (tptc_logprobs)."""
+    check(lib().tptc_logprobs(type_, _ptr(d_logits), rows, vocab, row_stride, _opt(d_token), _opt(d_logprob),
+                              _opt(d_entropy), n_top, _opt(d_top_id), _opt(d_top_logprob), stream))

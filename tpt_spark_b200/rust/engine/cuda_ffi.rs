@@ -38,6 +38,7 @@ pub const TPTC_TYPE_Q3_K: c_int = 11;
 pub const TPTC_TYPE_Q4_K: c_int = 12;
 pub const TPTC_TYPE_Q5_K: c_int = 13;
 pub const TPTC_TYPE_Q6_K: c_int = 14;
+pub const TPTC_TYPE_BF16: c_int = 30;
 
 pub const TPTC_SHARD_Q: c_int = 0;
 pub const TPTC_SHARD_K: c_int = 1;
@@ -50,6 +51,33 @@ pub const TPTC_SHARD_DOWN: c_int = 6;
 pub const TPTC_FUSED_NEVER: c_int = 0;
 pub const TPTC_FUSED_AUTO: c_int = 1;
 pub const TPTC_FUSED_ALWAYS: c_int = 2;
+
+/// A paged 8-bit KV cache over the caller's device buffers (kernel-level entry points).
+#[repr(C)]
+pub struct tptc_kv8 {
+    pub k: *mut i8,
+    pub v: *mut i8,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+    pub table: *const i32,
+    pub status: *mut i32,
+    pub n_pages: i32,
+    pub page: i32,
+    pub n_kv: i32,
+    pub head_dim: i32,
+    pub n_seq: i32,
+    pub max_pages: i32,
+}
+
+/// Rotary tables on the device.
+#[repr(C)]
+pub struct tptc_rope {
+    pub cos: *const f32,
+    pub sin: *const f32,
+    pub rows: i32,
+    pub dim: i32,
+    pub halves: i32,
+}
 
 /// Opaque engine context (one per GPU; one host thread at a time).
 #[repr(C)]
@@ -182,4 +210,15 @@ extern "C" {
                                     head_dim: c_int, max_seq: c_int, d_out: *mut f32,
                                     stream: *mut c_void) -> c_int;
     pub fn tptc_attn_decode_noalloc_status(stream: *mut c_void, out_code: *mut c_int) -> c_int;
+    // No counterpart in the reference: batched serving over a paged 8-bit KV cache.
+    pub fn tptc_kv8_append(cache: *const tptc_kv8, rope: *const tptc_rope, type_: c_int, d_q: *const c_void,
+                           q_stride: i64, d_k: *const c_void, k_stride: i64, d_v: *const c_void, v_stride: i64,
+                           n_heads: c_int, d_q_out: *mut c_void, d_k_out: *mut c_void, d_cu: *const i32,
+                           d_start: *const i32, n_tokens: c_int, max_new: c_int, stream: *mut c_void) -> c_int;
+    pub fn tptc_kv8_read(cache: *const tptc_kv8, type_: c_int, d_cu: *const i32, d_start: *const i32,
+                         n_tokens: c_int, max_rows: c_int, d_k_out: *mut c_void, d_v_out: *mut c_void,
+                         stream: *mut c_void) -> c_int;
+    pub fn tptc_logprobs(type_: c_int, d_logits: *const c_void, rows: c_int, vocab: c_int, row_stride: i64,
+                         d_token: *const i32, d_logprob: *mut f32, d_entropy: *mut f32, n_top: c_int,
+                         d_top_id: *mut i32, d_top_logprob: *mut f32, stream: *mut c_void) -> c_int;
 }
