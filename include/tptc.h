@@ -398,6 +398,18 @@ TPTC_API int tptc_kv8_append(const tptc_kv8* cache, const tptc_rope* rope, int t
 TPTC_API int tptc_kv8_read(const tptc_kv8* cache, int type, const int32_t* d_cu, const int32_t* d_start,
                            int n_tokens, int max_rows, void* d_k_out, void* d_v_out, void* stream);
 
+/* Attention of one query row per sequence over its first d_len[b] cached positions (the decode
+ * step of a batch; append the step's key and value first).
+ *   d_q: rotated queries of `type`, sequence b at element b * q_stride, [n_heads][head_dim];
+ *   d_out: [n_seq][n_heads][head_dim] of `type` = softmax(q.k / sqrt(head_dim)) . V, query head h reading
+ *     kv head h / (n_heads / n_kv).  A sequence of length 0 gets zeros.
+ * d_workspace holds tptc_kv8_attn_workspace_bytes() bytes (for the current device) and must be zero
+ * before its first use; each call leaves it ready for the next.  Calls that may overlap on
+ * the GPU need separate workspaces.  Results do not depend on scheduling. */
+TPTC_API int64_t tptc_kv8_attn_workspace_bytes(const tptc_kv8* cache, int n_heads);
+TPTC_API int tptc_kv8_attn(const tptc_kv8* cache, int type, const void* d_q, int64_t q_stride, const int32_t* d_len,
+                           int n_heads, void* d_out, void* d_workspace, int64_t workspace_bytes, void* stream);
+
 /* Log probabilities of given tokens beside tptc_sample, in one pass over the logits: rows of `vocab` logits of
  * `type`, row r at element r * row_stride (any alignment of whole elements).
  *   d_logprob[r] = log softmax(row)[d_token[r]] (both NULL: not wanted; an id outside the

@@ -69,7 +69,28 @@ def test_reads(code, kw):
     refused(code, read, **kw)
 
 
+def attn(c=None, **kw):
+    a = dict(d_q=P, q_stride=256, type_=K.F16, d_len=P, n_heads=4, d_out=P, d_workspace=P, workspace_bytes=1 << 30)
+    a.update(kw)
+    (c or cache()).attn(**a)
+
+
+@pytest.mark.parametrize("code,kw", [
+    (UNSUPPORTED, dict(type_=14)), (ARG, dict(d_q=0)), (ARG, dict(d_len=0)), (ARG, dict(d_out=0)), (ARG, dict(d_workspace=0)),
+    (ARG, dict(n_heads=3)), (ARG, dict(n_heads=0)), (ARG, dict(q_stride=255)), (ARG, dict(q_stride=260)), (ARG, dict(d_q=P + 8)),
+    (ARG, dict(d_out=P + 2)), (ARG, dict(d_workspace=P + 4))])
+def test_attentions(code, kw):
+    refused(code, attn, **kw)
+
+
+def test_attention_caches():
+    refused(UNSUPPORTED, attn, cache(head_dim=80))
+    refused(ARG, attn, cache(n_seq=1 << 30))
+    refused(ARG, cache().attn_workspace_bytes, 5)
+
+
 def test_nothing_to_do_is_no_error():
+    attn(cache(n_seq=0))
     append(n_tokens=0)
     append(max_new=0)
     append(cache(n_seq=0))

@@ -685,6 +685,49 @@ TPTC_API int tptc_kv8_read(const tptc_kv8* cache, int type, const int32_t* d_cu,
     return e == cudaSuccess ? TPTC_OK : cuda_fail(e, "kv8_read");
 }
 
+// Whether n_heads query heads fit the cache (the workspace's sizes stay within 31 bits of counters).
+static int kv8_attn_args(const tptc_kv8* c, int type, int n_heads) {
+    if (int rc = kv8_args(c, type)) return rc;
+    if (n_heads <= 0 || n_heads % c->n_kv)
+        return fail_code(nullptr, TPTC_ERR_ARG, "kv8_attn: n_heads must be a positive multiple of n_kv");
+    if ((int64_t)c->n_seq * n_heads > INT32_MAX) return fail_code(nullptr, TPTC_ERR_ARG, "kv8_attn: too many sequences");
+    return TPTC_OK;
+}
+
+TPTC_API int64_t tptc_kv8_attn_workspace_bytes(const tptc_kv8* cache, int n_heads) {
+    if (int rc = kv8_attn_args(cache, TPTC_TYPE_F16, n_heads)) return rc;
+    int dev = 0, sms = 0;
+    if (int rc = ensure_kernels(&dev, &sms)) return rc;
+    return (int64_t)tptc::kv8_attn_workspace(*cache, n_heads, sms);
+}
+
+TPTC_API int tptc_kv8_attn(const tptc_kv8* cache, int type, const void* d_q, int64_t q_stride, const int32_t* d_len,
+                           int n_heads, void* d_out, void* d_workspace, int64_t workspace_bytes, void* stream) {
+    if (int rc = kv8_attn_args(cache, type, n_heads)) return rc;
+    if (!d_q || !d_len || !d_out || !d_workspace) return fail_code(nullptr, TPTC_ERR_ARG, "kv8_attn: null pointer");
+    if (bad_rows(d_q, q_stride, (int64_t)n_heads * cache->head_dim, type) || misaligned(d_out, 16) ||
+        misaligned(d_workspace, 16))
+        return fail_code(nullptr, TPTC_ERR_ARG, "kv8_attn: q rows, out and workspace must be 16-byte aligned");
+    if (cache->n_seq == 0) return TPTC_OK;
+    int dev = 0, sms = 0;
+    if (int rc = ensure_kernels(&dev, &sms)) return rc;
+    const size_t need = tptc::kv8_attn_workspace(*cache, n_heads, sms);
+    if (workspace_bytes < (int64_t)need)
+        return fail_code(nullptr, TPTC_ERR_ARG,
+                         "kv8_attn: workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) +
+                             " needed");
+    tptc::Kv8Attn p = {};
+    p.c = *cache;
+    p.q = d_q;
+    p.q_stride = q_stride;
+    p.len = d_len;
+    p.n_heads = n_heads;
+    p.out = d_out;
+    p.workspace = static_cast<uint8_t*>(d_workspace);
+    cudaError_t e = tptc::launch_kv8_attn(type, p, sms, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? TPTC_OK : cuda_fail(e, "kv8_attn");
+}
+
 TPTC_API int tptc_logprobs(int type, const void* d_logits, int rows, int vocab, int64_t row_stride,
                            const int32_t* d_token, float* d_logprob, float* d_entropy, int n_top, int32_t* d_top_id,
                            float* d_top_logprob, void* stream) {

@@ -334,6 +334,10 @@ cudaError_t launch_kv8_read(int type, Kv8Read p, cudaStream_t st) {
     return read_t<float>(p, ctas, st);
 }
 
-cudaError_t serve_init_device() { return logprobs_init_device(); }
+cudaError_t serve_init_device() {
+    cudaError_t e = logprobs_init_device();
+    if (e == cudaSuccess) e = kv8_attn_init_device();
+    return e;
+}
 
 }  // namespace tptc

@@ -1,0 +1,585 @@
+// kv8_attn.cu -- attention of one query row per sequence over the paged 8-bit KV cache.
+//
+// For key j of block (page, kv head) with scales ks, vs and codes c, d:
+//     s_j = (q . c_j) ks / sqrt(hd),     out = sum_j softmax(s)_j vs d_j.
+// Codes are integers up to 127, exact in fp16, so both products run on the tensor cores against
+// the codes themselves and each scale multiplies a 16-key tile's scores and weights afterwards.
+//
+// Bound: every K and V byte is read once for the whole head group (HBM).  What the layout is
+// built around is therefore bytes in flight: 16 keys are one m16n8k16 step with the keys as M, so
+// the 8 columns carry up to 8 query heads,
+//     S^T[key][head] = K . Q^T,          O^T[dim][head] += V^T . P^T,
+// and the k indices of S and the dims of O are permuted so that each thread needs whole 16-byte
+// runs of the codes.  A thread copies exactly the bytes it will use itself (cp.async into its own slots
+// of a ring), so the loop has no barrier at all: a warp waits for its own copies only.
+//
+// Work split: the 16-key tiles of all (sequence, kv head) pairs form one line, cut into equal
+// ranges, one per CTA, so ragged batches are balanced whatever the lengths; inside a range the
+// warps take every kWarps-th tile.  A pair that several CTAs share is joined by the last of them (a
+// ticket per pair), adding the parts in CTA order: results do not depend on scheduling.
+//
+// Weights: p = 2^(x - m) with a reference m that moves only when a score passes it by 8 (f32 sum
+// l).  The tensor core takes p vs 2^(m - M) as fp16, where M is the same kind of reference for
+// x + log2 vs: pages whose scales differ by any ratio keep fp16's relative precision against the
+// largest contribution.  For f32 queries q and the weights go in as a high and a low fp16 part.
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "serve.h"
+
+namespace tptc {
+
+namespace {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kStages = 3;
+constexpr int kCtasPerSm = 4;
+constexpr int kTile = 16;       // keys
+constexpr int kHeads = 8;       // query heads per pass over the keys (columns of the products)
+constexpr int kMinTiles = 16;   // tiles that make a CTA worth its share of the join
+
+template <int HD>
+struct Lay {
+    static constexpr int kKVec = HD == 96 ? 8 : 16;   // bytes per copy of K
+    static constexpr int kKPer = HD / 4 / kKVec;      // copies per row and thread
+    static constexpr int kVVec = HD == 128 ? 16 : HD == 96 ? 4 : 8;
+    static constexpr int kVPer = HD / 8 / kVVec;
+    static constexpr int kKBytes = kTile * HD;
+    static constexpr int kStage = 2 * kKBytes;
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kRecord = 3 * kHeads + kHeads * HD;  // floats: m, l, M, O of one part
+    static constexpr int kJoin = kWarps * kRecord * 4;
+    static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+};
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+
+template <int BYTES>
+__device__ __forceinline__ void lds(uint32_t (&w)[BYTES / 4], uint32_t addr) {
+    if constexpr (BYTES == 16)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+    else if constexpr (BYTES == 8)
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+    else
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Bytes 0, 1 (HI: 2, 3) of a word of codes + 128 as fp16 codes: 1024 + byte is exact, so is the difference.
+template <bool HI>
+__device__ __forceinline__ uint32_t codes2(uint32_t w) {
+    const uint32_t h = __byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140);
+    const uint32_t off = 0x64806480u;  // 1152, 1152
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&off));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float (&x)[4]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        const T *a = reinterpret_cast<const T*>(&v.x), *b = reinterpret_cast<const T*>(&v.y);
+        x[0] = to_f32(a[0]), x[1] = to_f32(a[1]), x[2] = to_f32(b[0]), x[3] = to_f32(b[1]);
+    }
+}
+
+struct Params {
+    tptc_kv8 c;
+    const void* q;
+    int64_t q_stride;
+    const int32_t* len;
+    int n_heads;
+    void* out;
+    int* counters;   // [n_seq * pairs per sequence], zero between calls
+    float* records;  // [2 * grid]
+    float scale_log2;
+};
+
+// Length of a sequence (0: nothing, or out of range).
+__device__ __forceinline__ int length_of(const Params& p, int b, bool report) {
+    const int n = p.len[b];
+    if (n < 0 || n > p.c.max_pages * p.c.page) {
+        if (report && p.c.status) atomicExch(p.c.status, TPTC_ERR_ARG);
+        return 0;
+    }
+    return n;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __grid_constant__ Params p) {
+    using L = Lay<HD>;
+    constexpr bool kSplit = sizeof(T) == 4;  // high and low parts
+    constexpr int KS = HD / 16, MT = HD / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int s_scan[kWarps], s_start[3];
+    __shared__ int s_last;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int G = p.n_heads / p.c.n_kv, subs = (G + kHeads - 1) / kHeads, pairs = p.c.n_kv * subs;
+
+    // ---- this CTA's range of the line of tiles
+    int64_t total = 0;
+    for (int b0 = 0; b0 < p.c.n_seq; b0 += kThreads) {
+        const int b = b0 + tid;
+        int t = b < p.c.n_seq ? (length_of(p, b, blockIdx.x == 0) + kTile - 1) / kTile : 0;
+        t = warp_sum_i(t);
+        __syncthreads();
+        if (lane == 0) s_scan[warp] = t;
+        __syncthreads();
+        for (int w = 0; w < kWarps; w++) total += s_scan[w];
+    }
+    // sequences without a position: zeros
+    for (int b = blockIdx.x; b < p.c.n_seq; b += gridDim.x)
+        if (length_of(p, b, false) == 0)
+            for (int i = tid; i < p.n_heads * HD; i += kThreads)
+                static_cast<T*>(p.out)[(int64_t)b * p.n_heads * HD + i] = static_cast<T>(0.f);
+    total *= pairs;
+    const int64_t ctas = min((int64_t)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
+    if (blockIdx.x >= ctas) return;
+    int64_t at = blockIdx.x * total / ctas;
+    const int64_t end = (blockIdx.x + 1) * total / ctas, first = at;
+    {
+        int64_t before = 0;  // tiles before the block of sequences
+        bool found = false;
+        for (int b0 = 0; b0 < p.c.n_seq && !found; b0 += kThreads) {
+            const int b = b0 + tid;
+            const int t = b < p.c.n_seq ? (length_of(p, b, false) + kTile - 1) / kTile : 0;
+            int incl = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            __syncthreads();
+            if (lane == 31) s_scan[warp] = incl;
+            __syncthreads();
+            int64_t lead = before;
+            for (int w = 0; w < warp; w++) lead += s_scan[w];
+            const int64_t lo = (lead + incl - t) * pairs, hi = (lead + incl) * pairs;
+            const bool mine = t > 0 && lo <= at && at < hi;
+            if (mine) {
+                s_start[0] = b;
+                s_start[1] = (int)((at - lo) / t);
+                s_start[2] = (int)((at - lo) % t);
+            }
+            found = __syncthreads_or(mine);
+            for (int w = 0; w < kWarps; w++) before += s_scan[w];
+        }
+    }
+    int b = s_start[0], pair = s_start[1], tile = s_start[2];
+    int len = length_of(p, b, false), tiles = (len + kTile - 1) / kTile;
+
+    const uint32_t ring = smem_u32(smem) + warp * (kStages * L::kStage);
+    for (; at < end;) {
+        const int n = (int)min((int64_t)(tiles - tile), end - at);  // tiles of this piece
+        const int kvh = pair / subs, h0 = kvh * G + (pair % subs) * kHeads, nh = min(kHeads, kvh * G + G - h0);
+
+        // ---- the queries, as the B operand: thread holds head g, dims of its own bytes of K
+        uint32_t qh[KS][2], ql[kSplit ? KS : 1][2];
+        float fq0, fq1;
+        {
+            const T* q = static_cast<const T*>(p.q) + (int64_t)b * p.q_stride + (int64_t)(h0 + g) * HD;
+            float x[KS][4], top = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                constexpr int per = L::kKVec / 4;  // k steps per copy
+                const int d = (s / per) * (4 * L::kKVec) + t4 * L::kKVec + (s % per) * 4;
+                x[s][0] = x[s][1] = x[s][2] = x[s][3] = 0.f;
+                if (g < nh) load4(q + d, x[s]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[s][e]));
+            }
+            // a power of two that brings the largest element to [1, 2): fp16 then holds bf16 exactly
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            int e2 = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0 : (int)(__float_as_uint(top) >> 23) - 127;
+            if (!(top <= 3.402823466e38f) || top < 1.17549435e-38f) e2 = 0;
+            const float down = ldexpf(1.f, -e2);
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float a = x[s][2 * i] * down, c = x[s][2 * i + 1] * down;
+                    qh[s][i] = pack2<__half>(a, c);
+                    if constexpr (kSplit) {
+                        const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&qh[s][i]));
+                        ql[s][i] = pack2<__half>(a - hi.x, c - hi.y);
+                    }
+                }
+            }
+            const float f = ldexpf(p.scale_log2, e2);
+            fq0 = __shfl_sync(0xffffffffu, f, 8 * t4);
+            fq1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
+        }
+
+        // ---- page ids and scales: lane i holds those of this warp's tile 32 * batch + i
+        const int mine = n > warp ? (n - warp + kWarps - 1) / kWarps : 0;  // tiles of this warp
+        const int32_t* table = p.c.table + (int64_t)b * p.c.max_pages;
+        auto fetch = [&](int batch, int& id, float& ks, float& vs) {
+            const int i = 32 * batch + lane;
+            id = 0;
+            ks = vs = 0.f;
+            if (i < mine) {
+                const int64_t pos = (int64_t)(tile + warp + i * kWarps) * kTile;
+                id = table[pos / p.c.page];
+                if (id >= 0 && id < p.c.n_pages) {
+                    const int64_t k = (int64_t)id * p.c.n_kv + kvh;
+                    ks = p.c.k_scale[k];
+                    vs = p.c.v_scale[k];
+                } else {  // not in the cache: not followed
+                    if (p.c.status) atomicExch(p.c.status, TPTC_ERR_ARG);
+                    id = 0;
+                    ks = vs = __int_as_float(0x7fc00000);
+                }
+            }
+        };
+        int id0, id1;
+        float ks0, vs0, ks1, vs1;
+        fetch(0, id0, ks0, vs0);
+        fetch(1, id1, ks1, vs1);
+        int batch = 0;  // id0 .. are of this batch, id1 .. of the next
+
+        auto issue = [&](int i) {
+            if (i < mine) {
+                const int id = __shfl_sync(0xffffffffu, (i >> 5) == batch ? id0 : id1, i & 31);
+                const int64_t pos = (int64_t)(tile + warp + i * kWarps) * kTile;
+                const int64_t row = ((int64_t)id * p.c.n_kv + kvh) * p.c.page + pos % p.c.page;
+                const int8_t* k = p.c.k + row * HD;
+                const int8_t* v = p.c.v + row * HD;
+                const uint32_t st = ring + (i % kStages) * L::kStage;
+#pragma unroll
+                for (int r = 0; r < 2; r++)
+#pragma unroll
+                    for (int j = 0; j < L::kKPer; j++)
+                        copy_async<L::kKVec>(st + ((r * L::kKPer + j) * 32 + lane) * L::kKVec,
+                                             k + (g + 8 * r) * HD + (j * 4 + t4) * L::kKVec);
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int j = 0; j < L::kVPer; j++)
+                        copy_async<L::kVVec>(st + L::kKBytes + ((r * L::kVPer + j) * 32 + lane) * L::kVVec,
+                                             v + (2 * t4 + (r & 1) + 8 * (r >> 1)) * HD + g * (HD / 8) + j * L::kVVec);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+
+        float o[MT][4];
+#pragma unroll
+        for (int j = 0; j < MT; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // heads 2 t4 and 2 t4 + 1
+        float r0 = -INFINITY, r1 = -INFINITY, w0 = 0.f, w1 = 0.f;   // M, and 2^(m - M)
+#pragma unroll
+        for (int i = 0; i < kStages - 1; i++) issue(i);
+
+        for (int i = 0; i < mine; i++) {
+            if ((i >> 5) != batch) {
+                batch++;
+                id0 = id1, ks0 = ks1, vs0 = vs1;
+                fetch(batch + 1, id1, ks1, vs1);
+            }
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            const float ks = __shfl_sync(0xffffffffu, ks0, i & 31), vs = __shfl_sync(0xffffffffu, vs0, i & 31);
+            const uint32_t st = ring + (i % kStages) * L::kStage;
+
+            // S^T: rows g and g + 8 are keys
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < L::kKPer; j++) {
+                uint32_t a[L::kKVec / 4], c[L::kKVec / 4];
+                lds<L::kKVec>(a, st + (j * 32 + lane) * L::kKVec);
+                lds<L::kKVec>(c, st + ((L::kKPer + j) * 32 + lane) * L::kKVec);
+#pragma unroll
+                for (int e = 0; e < L::kKVec / 4; e++) {
+                    const uint32_t wa = a[e] ^ 0x80808080u, wc = c[e] ^ 0x80808080u;
+                    const uint32_t f[4] = {codes2<false>(wa), codes2<false>(wc), codes2<true>(wa), codes2<true>(wc)};
+                    const int k = j * (L::kKVec / 4) + e;
+                    mma(s, f, qh[k][0], qh[k][1]);
+                    if constexpr (kSplit) mma(s, f, ql[k][0], ql[k][1]);
+                }
+            }
+            const int key = (tile + warp + i * kWarps) * kTile + g;
+            const bool in0 = key < len, in1 = key + 8 < len;
+            const float x0 = in0 ? s[0] * (ks * fq0) : -INFINITY, x1 = in0 ? s[1] * (ks * fq1) : -INFINITY;
+            const float x2 = in1 ? s[2] * (ks * fq0) : -INFINITY, x3 = in1 ? s[3] * (ks * fq1) : -INFINITY;
+            const float t0 = fmaxf(x0, x2), t1 = fmaxf(x1, x3);
+            // (a NaN score never moves a reference; it reaches l and O below)
+            const float lim0 = vs * w0 * ex2(t0 - m0), lim1 = vs * w1 * ex2(t1 - m1);
+            if (__any_sync(0xffffffffu, t0 > m0 + 8.f || t1 > m1 + 8.f || !(lim0 <= 256.f) || !(lim1 <= 256.f) ||
+                                           (vs > 0.f && (r0 == -INFINITY || r1 == -INFINITY)))) {
+                float c0 = t0, c1 = t1;
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                    c0 = fmaxf(c0, __shfl_xor_sync(0xffffffffu, c0, d));
+                    c1 = fmaxf(c1, __shfl_xor_sync(0xffffffffu, c1, d));
+                }
+                const float lv = lg2(vs);
+                auto move = [&](float c, float& m, float& l, float& r, float& w) {
+                    const float mn = fmaxf(m, c), rn = fmaxf(r, c + lv);
+                    l *= m == mn ? 1.f : ex2(m - mn);
+                    const float beta = r == rn ? 1.f : ex2(r - rn);
+                    m = mn, r = rn;
+                    w = rn == -INFINITY ? 0.f : ex2(fminf(mn - rn, 127.f));
+                    return beta;
+                };
+                const float b0 = move(c0, m0, l0, r0, w0), b1 = move(c1, m1, l1, r1, w1);
+#pragma unroll
+                for (int j = 0; j < MT; j++) o[j][0] *= b0, o[j][1] *= b1, o[j][2] *= b0, o[j][3] *= b1;
+            }
+            const float p0 = ex2(x0 - m0), p1 = ex2(x1 - m1), p2 = ex2(x2 - m0), p3 = ex2(x3 - m1);
+            l0 += p0 + p2;
+            l1 += p1 + p3;
+            const float v0 = vs * w0, v1 = vs * w1;
+            uint32_t bh[2], bl[2];
+            {
+                const float y0 = p0 * v0, y1 = p1 * v1, y2 = p2 * v0, y3 = p3 * v1;
+                const uint32_t ha = pack2<__half>(y0, y1), hb = pack2<__half>(y2, y3);
+                bh[0] = transpose8x8(ha);
+                bh[1] = transpose8x8(hb);
+                if constexpr (kSplit) {
+                    const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&ha));
+                    const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
+                    bl[0] = transpose8x8(pack2<__half>(y0 - fa.x, y1 - fa.y));
+                    bl[1] = transpose8x8(pack2<__half>(y2 - fb.x, y3 - fb.y));
+                }
+            }
+            // O^T: rows g and g + 8 of step j are dims 2 j and 2 j + 1 of the thread's bytes
+#pragma unroll
+            for (int j = 0; j < L::kVPer; j++) {
+                uint32_t v[4][L::kVVec / 4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) lds<L::kVVec>(v[r], st + L::kKBytes + ((r * L::kVPer + j) * 32 + lane) * L::kVVec);
+#pragma unroll
+                for (int e = 0; e < L::kVVec / 4; e++) {
+                    // keys 2 t4 and 2 t4 + 1 (+ 8) beside one another, dims 0 1 | 2 3
+                    uint32_t ab0 = __byte_perm(v[0][e], v[1][e], 0x5140) ^ 0x80808080u;
+                    uint32_t ab1 = __byte_perm(v[0][e], v[1][e], 0x7362) ^ 0x80808080u;
+                    uint32_t cd0 = __byte_perm(v[2][e], v[3][e], 0x5140) ^ 0x80808080u;
+                    uint32_t cd1 = __byte_perm(v[2][e], v[3][e], 0x7362) ^ 0x80808080u;
+                    const uint32_t f0[4] = {codes2<false>(ab0), codes2<true>(ab0), codes2<false>(cd0), codes2<true>(cd0)};
+                    const uint32_t f1[4] = {codes2<false>(ab1), codes2<true>(ab1), codes2<false>(cd1), codes2<true>(cd1)};
+                    const int k = 2 * (j * (L::kVVec / 4) + e);
+                    mma(o[k], f0, bh[0], bh[1]);
+                    mma(o[k + 1], f1, bh[0], bh[1]);
+                    if constexpr (kSplit) {
+                        mma(o[k], f0, bl[0], bl[1]);
+                        mma(o[k + 1], f1, bl[0], bl[1]);
+                    }
+                }
+            }
+            issue(i + kStages - 1);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+        }
+        __syncthreads();  // the ring becomes the join's memory
+
+        // ---- join the warps
+        float* rec = reinterpret_cast<float*>(smem);
+        {
+            float* me = rec + warp * L::kRecord;
+            if (g == 0) {
+                me[2 * t4] = m0, me[2 * t4 + 1] = m1;
+                me[kHeads + 2 * t4] = l0, me[kHeads + 2 * t4 + 1] = l1;
+                me[2 * kHeads + 2 * t4] = r0, me[2 * kHeads + 2 * t4 + 1] = r1;
+            }
+            float* mo = me + 3 * kHeads;
+#pragma unroll
+            for (int j = 0; j < MT; j++) {
+                float* a = mo + (2 * t4) * HD + g * (HD / 8) + 2 * j;
+                *reinterpret_cast<float2*>(a) = make_float2(o[j][0], o[j][2]);
+                *reinterpret_cast<float2*>(a + HD) = make_float2(o[j][1], o[j][3]);
+            }
+        }
+        __syncthreads();
+        const bool whole = n == tiles;
+        const int64_t piece0 = at - tile, piece1 = piece0 + tiles;  // the pair's part of the line
+        // slot 0 of the CTA: a pair that began before its range; 1: one that begins inside it
+        float* out_rec = p.records + (int64_t)(2 * blockIdx.x + (first >= piece0 ? 0 : 1)) * L::kRecord;
+        T* out = static_cast<T*>(p.out) + ((int64_t)b * p.n_heads + h0) * HD;
+
+        // out[h][d..] of `parts` records of rec(i), each scaled to the largest references; thread
+        // tid holds four dims of a head per step
+        auto ratio = [](float a, float m) { return a == m ? 1.f : ex2(a - m); };
+        for (int i = tid; i < kHeads * (HD / 4); i += kThreads) {
+            const int h = i / (HD / 4), d = (i % (HD / 4)) * 4;
+            float m = -INFINITY, r = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                m = fmaxf(m, rec[w * L::kRecord + h]);
+                r = fmaxf(r, rec[w * L::kRecord + 2 * kHeads + h]);
+            }
+            float l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                const float* a = rec + w * L::kRecord;
+                if (w >= n) break;  // a warp without a tile
+                l += a[kHeads + h] * ratio(a[h], m);
+                const float f = ratio(a[2 * kHeads + h], r);
+                const float4 v = *reinterpret_cast<const float4*>(a + 3 * kHeads + h * HD + d);
+                y[0] += v.x * f, y[1] += v.y * f, y[2] += v.z * f, y[3] += v.w * f;
+            }
+            if (whole) {
+                const float f = (r == -INFINITY ? 0.f : ex2(r - m)) / l;
+                if (h < nh)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) out[h * HD + d + e] = static_cast<T>(y[e] * f);
+            } else {
+                if (d == 0) out_rec[h] = m, out_rec[kHeads + h] = l, out_rec[2 * kHeads + h] = r;
+                *reinterpret_cast<float4*>(out_rec + 3 * kHeads + h * HD + d) = make_float4(y[0], y[1], y[2], y[3]);
+            }
+        }
+        if (!whole) {
+            const int64_t c0 = ((piece0 + 1) * ctas - 1) / total, c1 = (piece1 * ctas - 1) / total;
+            const int parts = (int)(c1 - c0 + 1);
+            int* counter = p.counters + (int64_t)b * pairs + pair;
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                s_last = atomicAdd(counter, 1) == parts - 1;
+                if (s_last) *counter = 0;
+                __threadfence();
+            }
+            __syncthreads();
+            if (s_last) {
+                auto part = [&](int i) {
+                    const int64_t c = c0 + i;
+                    return p.records + (2 * c + (c * total / ctas >= piece0 ? 0 : 1)) * L::kRecord;
+                };
+                for (int i = tid; i < kHeads * (HD / 4); i += kThreads) {
+                    const int h = i / (HD / 4), d = (i % (HD / 4)) * 4;
+                    if (h >= nh) continue;
+                    float m = -INFINITY, r = -INFINITY;
+                    for (int k = 0; k < parts; k++) {
+                        const float* a = part(k);
+                        m = fmaxf(m, __ldcg(a + h));
+                        r = fmaxf(r, __ldcg(a + 2 * kHeads + h));
+                    }
+                    float l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+                    for (int k = 0; k < parts; k++) {
+                        const float* a = part(k);
+                        l += __ldcg(a + kHeads + h) * ratio(__ldcg(a + h), m);
+                        const float f = ratio(__ldcg(a + 2 * kHeads + h), r);
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(a + 3 * kHeads + h * HD + d));
+                        y[0] += v.x * f, y[1] += v.y * f, y[2] += v.z * f, y[3] += v.w * f;
+                    }
+                    const float f = (r == -INFINITY ? 0.f : ex2(r - m)) / l;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) out[h * HD + d + e] = static_cast<T>(y[e] * f);
+                }
+            }
+        }
+        __syncthreads();  // the join's memory becomes the ring again
+
+        // ---- the next pair
+        at += n;
+        tile = 0;
+        if (++pair == pairs) {
+            pair = 0;
+            do {
+                if (++b >= p.c.n_seq) break;
+                len = length_of(p, b, false);
+            } while (len == 0);
+            tiles = (len + kTile - 1) / kTile;
+        }
+    }
+}
+
+int grid_of(int sms) { return kCtasPerSm * sms; }
+int pairs_of(int n_heads, int n_kv) { return n_kv * ceil_div(n_heads / n_kv, kHeads); }
+size_t counter_bytes(const tptc_kv8& c, int n_heads) {
+    return ((size_t)c.n_seq * pairs_of(n_heads, c.n_kv) * sizeof(int) + 255) / 256 * 256;
+}
+
+template <typename T, int HD>
+cudaError_t launch(const Params& p, int sms, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid_of(sms));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Lay<HD>::kSmem;
+    cfg.stream = st;
+    return cudaLaunchKernelEx(&cfg, kv8_attn_kernel<T, HD>, p);
+}
+
+template <typename T>
+cudaError_t launch_t(const Params& p, int sms, cudaStream_t st) {
+    if (p.c.head_dim == 64) return launch<T, 64>(p, sms, st);
+    if (p.c.head_dim == 96) return launch<T, 96>(p, sms, st);
+    return launch<T, 128>(p, sms, st);
+}
+
+template <typename T>
+cudaError_t init_t() {
+    cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<T, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<64>::kSmem);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kv8_attn_kernel<T, 96>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<96>::kSmem);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kv8_attn_kernel<T, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<128>::kSmem);
+    return e;
+}
+
+}  // namespace
+
+size_t kv8_attn_workspace(const tptc_kv8& c, int n_heads, int sms) {
+    return counter_bytes(c, n_heads) + (size_t)2 * grid_of(sms) * (3 * kHeads + kHeads * c.head_dim) * sizeof(float);
+}
+
+cudaError_t launch_kv8_attn(int type, const Kv8Attn& a, int sms, cudaStream_t st) {
+    Params p = {};
+    p.c = a.c;
+    p.q = a.q;
+    p.q_stride = a.q_stride;
+    p.len = a.len;
+    p.n_heads = a.n_heads;
+    p.out = a.out;
+    p.counters = reinterpret_cast<int*>(a.workspace);
+    p.records = reinterpret_cast<float*>(a.workspace + counter_bytes(a.c, a.n_heads));
+    p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)a.c.head_dim));
+    if (type == TPTC_TYPE_F16) return launch_t<__half>(p, sms, st);
+    if (type == TPTC_TYPE_BF16) return launch_t<__nv_bfloat16>(p, sms, st);
+    return launch_t<float>(p, sms, st);
+}
+
+cudaError_t kv8_attn_init_device() {
+    cudaError_t e = init_t<__half>();
+    if (e == cudaSuccess) e = init_t<__nv_bfloat16>();
+    if (e == cudaSuccess) e = init_t<float>();
+    return e;
+}
+
+}  // namespace tptc

@@ -90,6 +90,20 @@ struct Kv8Read {
 };
 cudaError_t launch_kv8_read(int type, Kv8Read p, cudaStream_t st);
 
+// kv8_attn.cu
+struct Kv8Attn {
+    tptc_kv8 c;
+    const void* q;
+    int64_t q_stride;
+    const int32_t* len;
+    int n_heads;
+    void* out;
+    uint8_t* workspace;  // kv8_attn_workspace() bytes; the counters at its head are zero between calls
+};
+size_t kv8_attn_workspace(const tptc_kv8& c, int n_heads, int sms);
+cudaError_t launch_kv8_attn(int type, const Kv8Attn& a, int sms, cudaStream_t st);
+cudaError_t kv8_attn_init_device();
+
 // logprobs.cu
 constexpr int kMaxTop = 32;
 struct LogprobParams {

@@ -162,6 +162,15 @@ class Kv8Cache:
         check(lib().tptc_kv8_read(self._h, type_, _ptr(d_cu), _ptr(d_start), n_tokens, max_rows, _opt(d_k_out),
                                   _opt(d_v_out), stream))
 
+    def attn_workspace_bytes(self, n_heads: int) -> int:
+        return check(lib().tptc_kv8_attn_workspace_bytes(self._h, n_heads))
+
+    def attn(self, d_q, q_stride: int, type_: int, d_len, n_heads: int, d_out, d_workspace, workspace_bytes: int,
+             stream: Optional[int] = None) -> None:
+        """Attention of one query row per sequence over its first d_len[b] positions (tptc_kv8_attn)."""
+        check(lib().tptc_kv8_attn(self._h, type_, _ptr(d_q), q_stride, _ptr(d_len), n_heads, _ptr(d_out),
+                                  _ptr(d_workspace), workspace_bytes, stream))
+
 
 def logprobs(d_logits, type_: int, rows: int, vocab: int, row_stride: int, d_token, d_logprob, d_entropy, n_top: int,
              d_top_id, d_top_logprob, stream: Optional[int] = None) -> None:

@@ -218,6 +218,10 @@ extern "C" {
     pub fn tptc_kv8_read(cache: *const tptc_kv8, type_: c_int, d_cu: *const i32, d_start: *const i32,
                          n_tokens: c_int, max_rows: c_int, d_k_out: *mut c_void, d_v_out: *mut c_void,
                          stream: *mut c_void) -> c_int;
+    pub fn tptc_kv8_attn_workspace_bytes(cache: *const tptc_kv8, n_heads: c_int) -> i64;
+    pub fn tptc_kv8_attn(cache: *const tptc_kv8, type_: c_int, d_q: *const c_void, q_stride: i64, d_len: *const i32,
+                         n_heads: c_int, d_out: *mut c_void, d_workspace: *mut c_void, workspace_bytes: i64,
+                         stream: *mut c_void) -> c_int;
     pub fn tptc_logprobs(type_: c_int, d_logits: *const c_void, rows: c_int, vocab: c_int, row_stride: i64,
                          d_token: *const i32, d_logprob: *mut f32, d_entropy: *mut f32, n_top: c_int,
                          d_top_id: *mut i32, d_top_logprob: *mut f32, stream: *mut c_void) -> c_int;
