@@ -410,6 +410,18 @@ TPTC_API int64_t tptc_kv8_attn_workspace_bytes(const tptc_kv8* cache, int n_head
 TPTC_API int tptc_kv8_attn(const tptc_kv8* cache, int type, const void* d_q, int64_t q_stride, const int32_t* d_len,
                            int n_heads, void* d_out, void* d_workspace, int64_t workspace_bytes, void* stream);
 
+/* Causal attention over packed prompts, TPTC_TYPE_F16 or TPTC_TYPE_BF16.  Sequence b has the query rows
+ * d_cu_q[b] .. d_cu_q[b + 1] of n_q and the keys d_cu_k[b] .. d_cu_k[b + 1] of n_k; its queries are the last
+ * of its key positions: query i of lq sees keys 0 .. lk - lq + i (a row that sees none gets
+ * zeros).  Rows: token t at element t * stride, heads adjacent; 16-byte aligned, strides multiples
+ * of 8 elements; d_out [n_q][n_heads][head_dim].  Any n_heads that is a multiple of n_kv, up to 128 query heads per kv
+ * head; head_dim 64, 96 or 128.  max_q: no sequence has more query rows.  K and V hold finite
+ * values (what lies behind the last key of a sequence is never used). */
+TPTC_API int tptc_attn_packed(int type, const void* d_q, int64_t q_stride, const void* d_k, int64_t k_stride,
+                              const void* d_v, int64_t v_stride, void* d_out, const int32_t* d_cu_q,
+                              const int32_t* d_cu_k, int n_seq, int n_q, int n_k, int max_q, int n_heads, int n_kv,
+                              int head_dim, int32_t* d_status, void* stream);
+
 /* Log probabilities of given tokens beside tptc_sample, in one pass over the logits: rows of `vocab` logits of
  * `type`, row r at element r * row_stride (any alignment of whole elements).
  *   d_logprob[r] = log softmax(row)[d_token[r]] (both NULL: not wanted; an id outside the

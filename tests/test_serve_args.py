@@ -89,7 +89,25 @@ def test_attention_caches():
     refused(ARG, cache().attn_workspace_bytes, 5)
 
 
+def packed(**kw):
+    a = dict(d_q=P, d_k=P, d_v=P, d_out=P, type_=K.F16, q_stride=256, k_stride=128, v_stride=128, d_cu_q=P, d_cu_k=P, n_seq=1,
+             n_q=10, n_k=10, max_q=10, n_heads=4, n_kv=2, head_dim=64)
+    a.update(kw)
+    K.attn_packed(**a)
+
+
+@pytest.mark.parametrize("code,kw", [
+    (UNSUPPORTED, dict(type_=K.F32)), (UNSUPPORTED, dict(head_dim=256)), (UNSUPPORTED, dict(n_heads=258, q_stride=1 << 20)),
+    (ARG, dict(n_heads=3)), (ARG, dict(n_kv=0)), (ARG, dict(n_heads=0)), (ARG, dict(n_seq=-1)), (ARG, dict(n_q=-1)),
+    (ARG, dict(n_k=-1)), (ARG, dict(max_q=-1)), (ARG, dict(n_k=2 ** 31 - 100)), (ARG, dict(d_q=0)), (ARG, dict(d_cu_k=0)),
+    (ARG, dict(d_out=P + 8)), (ARG, dict(q_stride=248)), (ARG, dict(k_stride=130)), (ARG, dict(d_v=P + 2))])
+def test_prompts(code, kw):
+    refused(code, packed, **kw)
+
+
 def test_nothing_to_do_is_no_error():
+    packed(n_seq=0)
+    packed(n_q=0)
     attn(cache(n_seq=0))
     append(n_tokens=0)
     append(max_new=0)

@@ -100,6 +100,8 @@ SIGNATURES = {
     "tptc_kv8_read": (c_int, [c_vp, c_int, c_vp, c_vp, c_int, c_int, c_vp, c_vp, c_vp]),
     "tptc_kv8_attn_workspace_bytes": (c_i64, [c_vp, c_int]),
     "tptc_kv8_attn": (c_int, [c_vp, c_int, c_vp, c_i64, c_vp, c_int, c_vp, c_vp, c_i64, c_vp]),
+    "tptc_attn_packed": (c_int, [c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int,
+                                 c_int, c_int, c_int, c_vp, c_vp]),
     "tptc_logprobs": (c_int, [c_int, c_vp, c_int, c_int, c_i64, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp]),
 }
 

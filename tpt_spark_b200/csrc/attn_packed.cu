@@ -1,0 +1,430 @@
+// attn_packed.cu -- causal attention over packed prompts of different lengths (tcgen05).
+//
+// Query i of a sequence with lq queries and lk keys sees keys 0 .. lk - lq + i.  For head h of
+// the group of kv head h / G:  S = Q K^T / sqrt(hd),  O = softmax(S) V.
+//
+// Tile: 128 TMEM lanes hold floor(128 / G) consecutive tokens x the G heads of one kv head, so every
+// lane is in use for short prompts too and a K/V tile is shared by the whole group.  A CTA owns two
+// such tiles, A and B, and streams 128-key tiles of K and V through one ring: while the
+// softmax warps of one tile work, the tensor core works for the other.
+// TMEM: S_A, S_B (128 columns each), O_A, O_B.  The weights P overwrite the scores' columns as
+// 16-bit pairs and enter the second product as its TMEM operand, so they never pass through shared
+// memory.  Per pair of tiles and 128 keys (hd 128): 2048 tensor cycles and, at 16 exponentials per
+// cycle and SM, 2048 exponential cycles: both bound it.
+//
+// Softmax: one thread per lane, base 2, with a reference maximum that moves (rescaling O in TMEM and
+// the f32 sum) only when a tile's maximum passes it by 8, so P stays below 2^8.
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "serve.h"
+#include "tcgen05.cuh"
+
+namespace tptc {
+
+namespace {
+
+constexpr int BM = 128, BN = 128;
+constexpr int kThreads = 384;  // warpgroup 0: copies (warp 0) and products (warp 1); 1 and 2: the softmax of A and B
+// Registers: 384 threads launch with 168 each; the softmax threads hold 128 scores and take what
+// warpgroup 0 gives back (128 x (56 + 2 x 216) <= 384 x 168).
+constexpr int kRegsFew = 56, kRegsMany = 216;
+constexpr int kTmemCols = 512;
+
+template <int HD>
+struct Lay {
+    static constexpr int NC = (HD + 63) / 64;          // 64-column blocks of a row (the last may be part empty)
+    static constexpr int kTileBytes = 128 * NC * 128;  // 128 rows of Q, K or V
+    static constexpr int kStages = HD == 64 ? 6 : 5;   // K and V tiles in turn
+    static constexpr int kKV = 2 * kTileBytes;
+    static constexpr int kBytes = kKV + kStages * kTileBytes;
+};
+
+struct Params {
+    void* out;
+    const int32_t *cu_q, *cu_k;
+    int n_seq, n_q, n_k, max_q, n_heads, n_kv, tokens;  // tokens per tile
+    float scale_log2;
+    int32_t* status;
+};
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// D += A B with A in TMEM.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+// 32 columns, not waited for; tmem_loaded() below ends the wait for all loads before it.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+          "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+          "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_loads_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Keeps the uses of loaded registers behind the wait.
+__device__ __forceinline__ void pin32(float* r) {
+    asm volatile("" : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]));
+    asm volatile("" : "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
+                 "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31]));
+}
+__device__ __forceinline__ void tmem_st32_async(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_stores_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two f32 fused multiply-adds or sums in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)),
+          "l"(reinterpret_cast<const unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_packed_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ Params p) {
+    using L = Lay<HD>;
+    constexpr int S = L::kStages, KS = HD / 16;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t q_full, full[S], empty[S], s_full[2], p_full[2], o_done[2], drain;
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = p.n_heads / p.n_kv;
+    // the pairs of tiles with the most keys first
+    const int per = p.n_kv * p.n_seq, pairs = gridDim.x / per;
+    const int pair = pairs - 1 - blockIdx.x / per, kvh = blockIdx.x % per % p.n_kv, b = blockIdx.x % per / p.n_kv;
+    const int q_lo = p.cu_q[b], q_hi = p.cu_q[b + 1], k_lo = p.cu_k[b], k_hi = p.cu_k[b + 1];
+    if (q_lo == q_hi) return;
+    if (q_lo < 0 || q_hi < q_lo || q_hi > p.n_q || q_hi - q_lo > p.max_q || k_lo < 0 || k_hi < k_lo || k_hi > p.n_k) {
+        if (pair == 0 && threadIdx.x == 0 && p.status) atomicExch(p.status, TPTC_ERR_ARG);
+        return;
+    }
+    const int lq = q_hi - q_lo, lk = k_hi - k_lo, tok0 = pair * 2 * p.tokens;
+    if (tok0 >= lq) return;
+    int toks[2], nt[2];  // tokens of a tile, and the key tiles that its last token sees
+    for (int t = 0; t < 2; t++) {
+        toks[t] = max(0, min(p.tokens, lq - tok0 - t * p.tokens));
+        const int sees = lk - lq + tok0 + t * p.tokens + toks[t];
+        nt[t] = toks[t] > 0 && sees > 0 ? (sees + BN - 1) / BN : 0;
+    }
+    const int ntot = max(nt[0], nt[1]);
+
+    if (threadIdx.x == 0) {
+        mbar_init(&q_full, 1);
+        for (int s = 0; s < S; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int t = 0; t < 2; t++) {
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_full[t], 4);  // one arrival per softmax warp
+            mbar_init(&o_done[t], 1);
+        }
+        mbar_init(&drain, 1);
+        fence_mbar_init();
+        abort_flag = 0;
+    }
+    if (warp == 1) tmem_alloc(&tmem_slot, kTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
+        if (warp == 0 && lane == 0 && ntot > 0) {  // copies: Q_A, Q_B, then K_0, V_0, K_1, ...
+            const uint32_t q_bytes = (uint32_t)(p.tokens * G) * 128 * L::NC;
+            mbar_expect_tx(&q_full, (toks[1] > 0 ? 2 : 1) * q_bytes);
+            for (int t = 0; t < 2; t++) {
+                if (toks[t] == 0) continue;
+#pragma unroll
+                for (int c = 0; c < L::NC; c++)
+                    tma_load_3d(smem + t * L::kTileBytes + c * BM * 128, &tq, c * 64, kvh * G, q_lo + tok0 + t * p.tokens,
+                                &q_full);
+            }
+            int i = 0;
+            for (; i < 2 * ntot; i++) {
+                const int s = i % S;
+                if (i >= S && !wait_or_abort(&empty[s], ((i / S) - 1) & 1, p.status, &abort_flag)) break;
+                mbar_expect_tx(&full[s], L::kTileBytes);
+#pragma unroll
+                for (int c = 0; c < L::NC; c++)
+                    tma_load_3d(smem + L::kKV + s * L::kTileBytes + c * BN * 128, (i & 1) ? &tv : &tk, c * 64, kvh,
+                                k_lo + (i >> 1) * BN, &full[s]);
+            }
+            // the copies still in flight land before the CTA exits
+            mbar_wait_bounded(&q_full, 0, nullptr);
+            for (int k = i > S ? i - S : 0; k < i; k++) mbar_wait_bounded(&full[k % S], (k / S) & 1, nullptr);
+        }
+        if (warp == 1 && lane == 0 && ntot > 0) {  // products
+            constexpr uint32_t type_bits = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+            const uint32_t id_s = mma_idesc(BM, BN) | type_bits, id_o = mma_idesc(BM, HD) | kIdescBMajorMN | type_bits;
+            auto slot = [&](int i) { return smem_u32(smem + L::kKV + (i % S) * L::kTileBytes); };
+            auto wait_full = [&](int i) { return wait_or_abort(&full[i % S], (i / S) & 1, p.status, &abort_flag); };
+            auto issue_s = [&](int t, int j) {
+                const uint32_t qa = smem_u32(smem + t * L::kTileBytes), ka = slot(2 * j);
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+                    mma_f16(tmem + BN * t, sw128_desc(qa + (k / 4) * BM * 128 + 32 * (k % 4)),
+                            sw128_desc(ka + (k / 4) * BN * 128 + 32 * (k % 4)), id_s, k != 0);
+                mma_commit(&s_full[t]);
+            };
+            auto issue_pv = [&](int t, int j) {
+                const uint32_t va = slot(2 * j + 1);
+#pragma unroll
+                for (int k = 0; k < BN / 16; k++)
+                    mma_ts(tmem + 256 + 128 * t, tmem + BN * t + 8 * k, sw128_desc_mn(va + k * 2048, BN * 128), id_o, (j | k) != 0);
+            };
+            bool ok = wait_or_abort(&q_full, 0, p.status, &abort_flag) && wait_full(0);
+            if (ok) {
+                tc_fence_after();
+                for (int t = 0; t < 2; t++)
+                    if (nt[t] > 0) issue_s(t, 0);
+                mma_commit(&empty[0]);
+            }
+            for (int j = 0; j < ntot && ok; j++) {
+                const bool more = j + 1 < ntot;
+                ok = wait_full(2 * j + 1) && (!more || wait_full(2 * j + 2));
+                for (int t = 0; t < 2 && ok; t++) {
+                    if (j >= nt[t]) continue;
+                    ok = wait_or_abort(&p_full[t], j & 1, p.status, &abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_pv(t, j);
+                    if (j + 1 < nt[t]) issue_s(t, j + 1);
+                    else mma_commit(&o_done[t]);
+                }
+                if (ok) {  // V_j and K_(j + 1) are used up
+                    mma_commit(&empty[(2 * j + 1) % S]);
+                    if (more) mma_commit(&empty[(2 * j + 2) % S]);
+                }
+            }
+            // every product issued has completed before TMEM is freed
+            mma_commit(&drain);
+            mbar_wait_bounded(&drain, 0, nullptr);
+        }
+    } else {  // one thread per lane of tile A or B
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
+        const int t = (warp >> 2) - 1, r = 32 * (warp & 3) + lane;
+        const uint32_t loff = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t tS = tmem + BN * t + loff, tO = tmem + 256 + 128 * t + loff;
+        const int tok = tok0 + t * p.tokens + min(r / G, max(toks[t] - 1, 0));  // spare lanes follow the last token
+        const int sees = lk - lq + tok + 1;                                  // keys of this lane
+        const int all_see = lk - lq + tok0 + t * p.tokens + 1;               // keys that every lane of the tile sees
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int j = 0; j < nt[t]; j++) {
+            ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[t], j & 1, p.status, &abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            float s[BN];
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) tmem_ld32_async(tS + c, s + c);
+            tmem_loads_done();
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) pin32(s + c);
+            if ((j + 1) * BN > all_see) {
+                const int left = sees - j * BN;
+#pragma unroll
+                for (int k = 0; k < BN; k++) s[k] = k < left ? s[k] : -INFINITY;
+            }
+            float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int k = 4; k < BN; k++) mx[k & 3] = fmaxf(mx[k & 3], s[k]);
+            const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+            const bool move = mt > m + 8.f;
+            float alpha = 1.f;
+            if (move) {
+                alpha = ex2(m - mt);
+                l *= alpha;
+                m = mt;
+            }
+            if (j > 0 && __any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    float o[32];
+                    uint32_t w[32];
+                    tmem_ld32_async(tO + c, o);
+                    tmem_loads_done();
+                    pin32(o);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) w[i] = __float_as_uint(o[i] * alpha);
+                    tmem_st32_async(tO + c, w);
+                }
+            }
+            const float neg = m == -INFINITY ? 0.f : -m;  // a lane that sees nothing yet: weights 0
+            const float2 sc = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int c = 0; c < BN; c += 64) {
+                uint32_t w[32];
+#pragma unroll
+                for (int k = 0; k < 32; k++) {
+                    const float2 y = fma2(make_float2(s[c + 2 * k], s[c + 2 * k + 1]), sc, off);
+                    const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                    sum[k & 1] = add2(sum[k & 1], e);
+                    w[k] = pack2<T>(e.x, e.y);
+                }
+                tmem_st32_async(tS + c / 2, w);
+            }
+            sum[0] = add2(sum[0], sum[1]);
+            l += sum[0].x + sum[0].y;
+            if ((j + 1) * BN > lk &&
+                __all_sync(0xffffffffu, wait_or_abort(&full[(2 * j + 1) % S], ((2 * j + 1) / S) & 1, p.status, &abort_flag))) {
+                // rows behind the sequence's last key may hold anything: zero them in V, so that
+                // weight 0 times them is 0 (both tiles write the same zeros, each before its product)
+                uint8_t* vb = smem + L::kKV + ((2 * j + 1) % S) * L::kTileBytes;
+                const int r0 = lk - j * BN, n = (BN - r0) * L::NC * 8;
+                for (int i = r; i < n; i += BM) {
+                    const int row = r0 + i / (L::NC * 8), rem = i % (L::NC * 8);
+                    *reinterpret_cast<uint4*>(vb + (rem >> 3) * BN * 128 + row * 128 + (rem & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+            }
+            tmem_stores_done();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[t]);
+        }
+        if (ok && nt[t] > 0) ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[t], 0, p.status, &abort_flag));
+        if (ok && toks[t] > 0) {
+            tc_fence_after();
+            const float il = l > 0.f || l != l ? 1.f / l : 0.f;
+            const bool mine = r < toks[t] * G;
+            T* row = static_cast<T*>(p.out) + ((int64_t)(q_lo + tok) * p.n_heads + kvh * G + r % G) * HD;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                float o[32];
+                if (nt[t] > 0) {
+                    tmem_ld32_async(tO + c, o);
+                    tmem_loads_done();
+                    pin32(o);
+                }
+                if (mine) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) w[i] = il == 0.f ? 0u : pack2<T>(o[2 * i] * il, o[2 * i + 1] * il);
+                    uint4* dst = reinterpret_cast<uint4*>(row + c);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+template <typename T, int HD>
+cudaError_t launch(const AttnPacked& a, const Params& p, cudaStream_t st) {
+    const int G = a.n_heads / a.n_kv;
+    CUtensorMap tq, tk, tv;
+    const bool bf = std::is_same<T, __nv_bfloat16>::value;
+    cudaError_t e = make_tmap_heads(&tq, a.q, bf, HD, a.n_heads, a.n_q, a.q_stride, G, p.tokens);
+    if (e == cudaSuccess && a.n_k > 0) e = make_tmap_heads(&tk, a.k, bf, HD, a.n_kv, a.n_k, a.k_stride, 1, BN);
+    if (e == cudaSuccess && a.n_k > 0) e = make_tmap_heads(&tv, a.v, bf, HD, a.n_kv, a.n_k, a.v_stride, 1, BN);
+    if (e != cudaSuccess) return e;
+    if (a.n_k == 0) tk = tv = tq;  // no key: no copy is made
+    const int64_t pairs = ceil_div64(std::min(a.max_q, a.n_q), 2 * p.tokens), ctas = pairs * a.n_kv * a.n_seq;
+    if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Lay<HD>::kBytes + 1024;
+    cfg.stream = st;
+    return cudaLaunchKernelEx(&cfg, attn_packed_kernel<T, HD>, tq, tk, tv, p);
+}
+
+template <typename T>
+cudaError_t launch_t(const AttnPacked& a, const Params& p, cudaStream_t st) {
+    if (a.head_dim == 64) return launch<T, 64>(a, p, st);
+    if (a.head_dim == 96) return launch<T, 96>(a, p, st);
+    return launch<T, 128>(a, p, st);
+}
+
+template <typename T>
+cudaError_t init_t() {
+    cudaError_t e = cudaFuncSetAttribute(attn_packed_kernel<T, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         Lay<64>::kBytes + 1024);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(attn_packed_kernel<T, 96>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<96>::kBytes + 1024);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(attn_packed_kernel<T, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 Lay<128>::kBytes + 1024);
+    return e;
+}
+
+}  // namespace
+
+cudaError_t attn_packed_init_device() {
+    cudaError_t e = init_t<__half>();
+    if (e == cudaSuccess) e = init_t<__nv_bfloat16>();
+    return e;
+}
+
+cudaError_t launch_attn_packed(int type, const AttnPacked& a, cudaStream_t st) {
+    Params p = {};
+    p.out = a.out;
+    p.cu_q = a.cu_q;
+    p.cu_k = a.cu_k;
+    p.n_seq = a.n_seq;
+    p.n_q = a.n_q;
+    p.n_k = a.n_k;
+    p.max_q = a.max_q;
+    p.n_heads = a.n_heads;
+    p.n_kv = a.n_kv;
+    p.tokens = BM / (a.n_heads / a.n_kv);
+    p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)a.head_dim));
+    p.status = a.status;
+    if (type == TPTC_TYPE_F16) return launch_t<__half>(a, p, st);
+    return launch_t<__nv_bfloat16>(a, p, st);
+}
+
+}  // namespace tptc

@@ -728,6 +728,50 @@ TPTC_API int tptc_kv8_attn(const tptc_kv8* cache, int type, const void* d_q, int
     return e == cudaSuccess ? TPTC_OK : cuda_fail(e, "kv8_attn");
 }
 
+TPTC_API int tptc_attn_packed(int type, const void* d_q, int64_t q_stride, const void* d_k, int64_t k_stride,
+                              const void* d_v, int64_t v_stride, void* d_out, const int32_t* d_cu_q,
+                              const int32_t* d_cu_k, int n_seq, int n_q, int n_k, int max_q, int n_heads, int n_kv,
+                              int head_dim, int32_t* d_status, void* stream) {
+    if (type != TPTC_TYPE_F16 && type != TPTC_TYPE_BF16)
+        return fail_code(nullptr, TPTC_ERR_UNSUPPORTED, "attn_packed: type must be TPTC_TYPE_F16 or _BF16");
+    if (head_dim != 64 && head_dim != 96 && head_dim != 128)
+        return fail_code(nullptr, TPTC_ERR_UNSUPPORTED, "attn_packed: head_dim must be 64, 96 or 128");
+    if (!d_q || !d_k || !d_v || !d_out || !d_cu_q || !d_cu_k)
+        return fail_code(nullptr, TPTC_ERR_ARG, "attn_packed: null pointer");
+    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv)
+        return fail_code(nullptr, TPTC_ERR_ARG, "attn_packed: n_heads must be a positive multiple of n_kv");
+    if (n_heads / n_kv > 128)
+        return fail_code(nullptr, TPTC_ERR_UNSUPPORTED, "attn_packed: up to 128 query heads per kv head");
+    if (n_seq < 0 || n_q < 0 || n_k < 0 || max_q < 0 || n_q > INT32_MAX - 512 || n_k > INT32_MAX - 512)
+        return fail_code(nullptr, TPTC_ERR_ARG, "attn_packed: bad row counts");
+    if (bad_rows(d_q, q_stride, (int64_t)n_heads * head_dim, type) || bad_rows(d_k, k_stride, (int64_t)n_kv * head_dim, type) ||
+        bad_rows(d_v, v_stride, (int64_t)n_kv * head_dim, type) || misaligned(d_out, 16))
+        return fail_code(nullptr, TPTC_ERR_ARG, "attn_packed: rows must be 16-byte aligned and not overlap");
+    if (n_seq == 0 || n_q == 0 || max_q == 0) return TPTC_OK;
+    int dev = 0, sms = 0;
+    if (int rc = ensure_kernels(&dev, &sms)) return rc;
+    tptc::AttnPacked p = {};
+    p.q = d_q;
+    p.k = d_k;
+    p.v = d_v;
+    p.q_stride = q_stride;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.out = d_out;
+    p.cu_q = d_cu_q;
+    p.cu_k = d_cu_k;
+    p.n_seq = n_seq;
+    p.n_q = n_q;
+    p.n_k = n_k;
+    p.max_q = max_q;
+    p.n_heads = n_heads;
+    p.n_kv = n_kv;
+    p.head_dim = head_dim;
+    p.status = d_status;
+    cudaError_t e = tptc::launch_attn_packed(type, p, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? TPTC_OK : cuda_fail(e, "attn_packed");
+}
+
 TPTC_API int tptc_logprobs(int type, const void* d_logits, int rows, int vocab, int64_t row_stride,
                            const int32_t* d_token, float* d_logprob, float* d_entropy, int n_top, int32_t* d_top_id,
                            float* d_top_logprob, void* stream) {

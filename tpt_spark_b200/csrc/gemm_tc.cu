@@ -218,6 +218,21 @@ cudaError_t make_tmap_f16(CUtensorMap* map, const __half* ptr, int64_t rows, int
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+cudaError_t make_tmap_heads(CUtensorMap* map, const void* ptr, bool bf16, int hd, int heads, int64_t rows,
+                            int64_t row_stride, int box_heads, int box_rows) {
+    cudaError_t e = get_encode();
+    if (e != cudaSuccess) return e;
+    const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)row_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = g_encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                                const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 cudaError_t gemm_tc_init_device() {
     cudaError_t e;
     if ((e = cudaFuncSetAttribute(gemm_tc_kernel<GEMM_STORE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem)))

@@ -337,6 +337,7 @@ cudaError_t launch_kv8_read(int type, Kv8Read p, cudaStream_t st) {
 cudaError_t serve_init_device() {
     cudaError_t e = logprobs_init_device();
     if (e == cudaSuccess) e = kv8_attn_init_device();
+    if (e == cudaSuccess) e = attn_packed_init_device();
     return e;
 }
 

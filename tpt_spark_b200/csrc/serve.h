@@ -104,6 +104,18 @@ size_t kv8_attn_workspace(const tptc_kv8& c, int n_heads, int sms);
 cudaError_t launch_kv8_attn(int type, const Kv8Attn& a, int sms, cudaStream_t st);
 cudaError_t kv8_attn_init_device();
 
+// attn_packed.cu
+struct AttnPacked {
+    const void *q, *k, *v;
+    int64_t q_stride, k_stride, v_stride;
+    void* out;
+    const int32_t *cu_q, *cu_k;
+    int n_seq, n_q, n_k, max_q, n_heads, n_kv, head_dim;
+    int32_t* status;
+};
+cudaError_t launch_attn_packed(int type, const AttnPacked& a, cudaStream_t st);
+cudaError_t attn_packed_init_device();
+
 // logprobs.cu
 constexpr int kMaxTop = 32;
 struct LogprobParams {

@@ -119,4 +119,10 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
 cudaError_t make_tmap_f16(CUtensorMap* map, const __half* ptr, int64_t rows, int64_t cols, int64_t ld,
                           int box_rows);
 
+// Host: rows of 16-bit elements [rows][heads][hd], `row_stride` elements apart with the heads
+// adjacent, as a 3-D tensor map (column, head, row) with a box of 64 columns x box_heads x box_rows
+// and 128-byte swizzle; what lies outside the tensor reads as zero (gemm_tc.cu).
+cudaError_t make_tmap_heads(CUtensorMap* map, const void* ptr, bool bf16, int hd, int heads, int64_t rows,
+                            int64_t row_stride, int box_heads, int box_rows);
+
 }  // namespace tptc

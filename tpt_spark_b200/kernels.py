@@ -172,6 +172,15 @@ class Kv8Cache:
                                   _ptr(d_workspace), workspace_bytes, stream))
 
 
+def attn_packed(d_q, d_k, d_v, d_out, type_: int, q_stride: int, k_stride: int, v_stride: int, d_cu_q, d_cu_k, n_seq: int,
+                n_q: int, n_k: int, max_q: int, n_heads: int, n_kv: int, head_dim: int, d_status=None,
+                stream: Optional[int] = None) -> None:
+    """Causal attention over packed prompts; queries are the last of their sequence's keys (tptc_attn_packed)."""
+    check(lib().tptc_attn_packed(type_, _ptr(d_q), q_stride, _ptr(d_k), k_stride, _ptr(d_v), v_stride, _ptr(d_out),
+                                 _ptr(d_cu_q), _ptr(d_cu_k), n_seq, n_q, n_k, max_q, n_heads, n_kv, head_dim,
+                                 _opt(d_status), stream))
+
+
 def logprobs(d_logits, type_: int, rows: int, vocab: int, row_stride: int, d_token, d_logprob, d_entropy, n_top: int,
              d_top_id, d_top_logprob, stream: Optional[int] = None) -> None:
     """Log probabilities of given tokens, entropy and the n_top largest of each row (tptc_logprobs)."""

@@ -222,6 +222,10 @@ extern "C" {
     pub fn tptc_kv8_attn(cache: *const tptc_kv8, type_: c_int, d_q: *const c_void, q_stride: i64, d_len: *const i32,
                          n_heads: c_int, d_out: *mut c_void, d_workspace: *mut c_void, workspace_bytes: i64,
                          stream: *mut c_void) -> c_int;
+    pub fn tptc_attn_packed(type_: c_int, d_q: *const c_void, q_stride: i64, d_k: *const c_void, k_stride: i64,
+                            d_v: *const c_void, v_stride: i64, d_out: *mut c_void, d_cu_q: *const i32,
+                            d_cu_k: *const i32, n_seq: c_int, n_q: c_int, n_k: c_int, max_q: c_int, n_heads: c_int,
+                            n_kv: c_int, head_dim: c_int, d_status: *mut i32, stream: *mut c_void) -> c_int;
     pub fn tptc_logprobs(type_: c_int, d_logits: *const c_void, rows: c_int, vocab: c_int, row_stride: i64,
                          d_token: *const i32, d_logprob: *mut f32, d_entropy: *mut f32, n_top: c_int,
                          d_top_id: *mut i32, d_top_logprob: *mut f32, stream: *mut c_void) -> c_int;
