@@ -6,16 +6,21 @@
 // A thread keeps (m, z, t) of its elements and moves them to a new maximum m' by
 // z <- z a, t <- a (t + z (m - m')), a = e^(m - m'); the CTA's states join in thread order.
 //
-// The n largest, exactly and with ties by lowest index: an element that beats the running
-// threshold goes to a shared buffer as one 64-bit key (ordered value bits, then ~index), which
-// makes keys unique and their order the wanted one.  The first threshold is the n-th largest of
-// 32 group maxima of the first chunk (n elements are at least that large); the buffer is
-// cut back to its n largest, which raises the threshold, when it fills.  After the first chunk
-// only about n ln(vocab / chunk) elements pass.
+// The n largest, exactly and with ties by lowest index.  An element is one 64-bit key (ordered
+// value bits, then ~index): keys are unique and their order is the wanted one.  Each warp keeps
+// its n largest sorted, lane i the i-th, and looks at a chunk's elements again only when one of
+// the 16-element maxima (which the online maximum needs anyway) reaches a threshold: the larger of
+// the warp's own n-th, of the n-th largest of the first chunk's 32 group maxima, and of the smallest
+// over the warps of their ceil(n / warps)-th, which they publish without a barrier (each bounds the
+// row's n-th from below, whenever it is read).  About n ln(vocab / chunk) elements of a row are
+// ever inserted.  (A shared candidate list with a barrier per chunk took 341 us for 1500 bf16 rows of 128256,
+// this takes 95 us; both with n = 5.)
 //
-// One CTA per row streams the logits (HBM bound); with few rows a cluster of 2, 4 or 8 CTAs
-// shares one row and joins through distributed shared memory (latency bound).
+// One CTA per row streams the logits: HBM bound, with the exponentials (16 per cycle and SM) close
+// behind for 16-bit logits.  With few rows a cluster of CTAs shares one row and joins through
+// distributed shared memory (latency bound).
 #include <algorithm>
+#include <type_traits>
 
 #include "serve.h"
 
@@ -23,11 +28,13 @@ namespace tptc {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kElems = 16;                   // elements per thread and chunk
-constexpr int kChunk = kThreads * kElems;
-constexpr int kLimit = 512;                  // buffered keys before they are cut back
-constexpr int kCap = kLimit + kChunk;        // a chunk can push every element
+constexpr int kThreads = 256;                // kWarps lists of up to 32 keys: also the cluster join's shape
+constexpr int kVecs = 4;                     // 16-byte vectors per thread and chunk
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxParts = 8;
+constexpr int kStages = 3;                   // chunks of the ring: two are on their way
+constexpr int kCtasPerSm = 4;
+constexpr int kRing = kStages * kVecs * kThreads * 16;
 
 __device__ __forceinline__ uint32_t ordered(float x) {
     if (isnan(x)) return 0xffffffffu;
@@ -43,89 +50,55 @@ __device__ __forceinline__ float unordered(uint32_t o) {
 struct State {
     float m, z, t;
 };
-// The state of two disjoint sets; an empty set has m = -inf, z = t = 0.
-__device__ __forceinline__ State join(const State& a, const State& b) {
-    const float m = fmaxf(a.m, b.m);
-    State r = {m, 0.f, 0.f};
-    const State* both[2] = {&a, &b};
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        if (both[i]->z == 0.f) continue;  // nothing with a probability (NaN is not 0)
-        const float d = both[i]->m - m, w = __expf(d);
-        r.z += both[i]->z * w;
-        r.t += w == 0.f ? 0.f : w * (both[i]->t + both[i]->z * d);
+// The state of the disjoint sets of the first `lanes` lanes (a power of two), in every one of
+// them; an empty set has m = -inf, z = t = 0.  The sums run in a fixed order.
+__device__ __forceinline__ State join_lanes(State s, int lanes) {
+    float m = s.m;
+    for (int o = 1; o < lanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float d = s.m - m, w = s.z == 0.f ? 0.f : __expf(d);  // (NaN is not 0)
+    float z = s.z * w, t = w == 0.f ? 0.f : w * (s.t + s.z * d);
+    for (int o = 1; o < lanes; o <<= 1) {
+        z += __shfl_xor_sync(0xffffffffu, z, o);
+        t += __shfl_xor_sync(0xffffffffu, t, o);
     }
-    return r;
+    return {m, z, t};
 }
 
 struct Shared {
-    unsigned long long key[kCap];
-    unsigned long long kept[2 * kLimit];
-    unsigned long long group[32];
-    unsigned long long bound;
-    State warp_state[kThreads / 32];
-    uint32_t group_max[32];
+    unsigned long long list[kWarps][kMaxTop];  // each warp's largest (a part's, in the cluster's join), descending
+    unsigned long long largest[kMaxTop];       // the CTA's
+    State warp_state[kWarps];
     State state;
-    float threshold;
-    int count, n_kept;
+    uint32_t group_max[32];
+    float first_threshold;
+    volatile float published[kWarps];
 };
 
-// Cuts key[0 .. count) back to its n largest, in descending order in key[0 ..); returns how
-// many there are.  Every thread of the CTA calls it; key is complete.
-__device__ int keep_largest(Shared& s, int count, int n) {
-    const int tid = threadIdx.x;
-    unsigned long long* list = s.key;
-    if (count > 64) {
-        // n of the 32 group maxima are at least the n-th of them: what is below is out
-        unsigned long long best = 0;
-        for (int i = tid; i < count; i += kThreads) best = max(best, s.key[i]);
+// The n largest of `lists` descending lists of kMaxTop keys (n of them used, the others 0), to
+// out[0 .. n) in order.  Keys that are not 0 are unique, and 0 stands for nothing.
+__device__ __forceinline__ void merge_lists(const unsigned long long (*list)[kMaxTop], int lists, int n,
+                                            unsigned long long* out) {
+    const int w = threadIdx.x / kMaxTop, i = threadIdx.x % kMaxTop;
+    if (w >= lists || i >= n) return;
+    const unsigned long long mine = list[w][i];
+    int before[kWarps];  // of list o, how many come before mine: a binary search, all lists at once
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-        if ((tid & 7) == 0) s.group[tid >> 3] = best;
-        if (tid == 0) s.n_kept = 0;
-        __syncthreads();
-        if (tid < 32) {
-            const unsigned long long mine = s.group[tid];
-            int rank = 0;
-            for (int i = 0; i < 32; i++) rank += s.group[i] > mine || (s.group[i] == mine && i < tid);
-            if (rank == n - 1) s.bound = mine;
-        }
-        __syncthreads();
-        const unsigned long long bound = s.bound;
-        for (int i = tid; i < count; i += kThreads)
-            if (s.key[i] >= bound) {
-                const int at = atomicAdd(&s.n_kept, 1);
-                if (at < 2 * kLimit) s.kept[at] = s.key[i];
-            }
-        __syncthreads();
-        if (s.n_kept <= 2 * kLimit) {
-            list = s.kept;
-            count = s.n_kept;
+    for (int o = 0; o < kWarps; o++) before[o] = 0;
+#pragma unroll
+    for (int step = kMaxTop / 2; step > 0; step >>= 1) {
+#pragma unroll
+        for (int o = 0; o < kWarps; o++) {
+            const unsigned long long k = list[o][before[o] + step - 1];
+            if (k > mine || (k == mine && o < w)) before[o] += step;
         }
     }
-    // ranks by counting (keys are unique); the largest n move to their places
-    if (list == s.key) {
-        constexpr int PER = (kCap + kThreads - 1) / kThreads;
-        unsigned long long mine[PER];
-        int rank[PER], k = 0;
-        for (int i = tid; i < count; i += kThreads, k++) {
-            mine[k] = s.key[i];
-            rank[k] = 0;
-            for (int j = 0; j < count; j++) rank[k] += s.key[j] > mine[k];
-        }
-        __syncthreads();
-        for (int i = 0; i < k; i++)
-            if (rank[i] < n) s.key[rank[i]] = mine[i];
-    } else {
-        for (int i = tid; i < count; i += kThreads) {
-            const unsigned long long mine = list[i];
-            int rank = 0;
-            for (int j = 0; j < count; j++) rank += list[j] > mine;
-            if (rank < n) s.key[rank] = mine;
-        }
+    int rank = i;
+#pragma unroll
+    for (int o = 0; o < kWarps; o++) {
+        const unsigned long long k = list[o][before[o]];  // the search ends one short of a whole list
+        if (o != w && o < lists) rank += before[o] + (k > mine || (k == mine && o < w));
     }
-    __syncthreads();
-    return min(count, n);
+    if (rank < n) out[rank] = mine;
 }
 
 __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
@@ -143,171 +116,253 @@ __device__ __forceinline__ float ld_peer_f32(uint32_t addr) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
     return v;
 }
-__device__ __forceinline__ int ld_peer_s32(uint32_t addr) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr));
-    return v;
-}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two f32 operations in one instruction.
+__device__ __forceinline__ unsigned long long bits(const float2& a) { return reinterpret_cast<const unsigned long long&>(a); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(bits(a)), "l"(bits(b)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(bits(a)), "l"(bits(b)));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// The two elements of a word, in f32.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constant__ LogprobParams p, int parts) {
-    constexpr int VEC = 16 / sizeof(T), U = kElems / VEC;
-    extern __shared__ __align__(16) uint8_t smem[];
-    Shared& s = *reinterpret_cast<Shared*>(smem);
-    const int tid = threadIdx.x, row = blockIdx.x / parts, part = blockIdx.x % parts, n = p.n_top;
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const __grid_constant__ LogprobParams p, int parts) {
+    constexpr int VEC = 16 / sizeof(T), U = kVecs, S = kStages, E = U * VEC, CHUNK = kThreads * E;
+    constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+    extern __shared__ __align__(16) uint8_t ring[];  // [S][U][kThreads] vectors, filled by the thread that sums them
+    __shared__ Shared s;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = blockIdx.x / parts, part = blockIdx.x % parts, n = p.n_top;
     const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.row_stride;
     // 16-byte vectors of memory: vector v holds elements v * VEC - shift ..; the parts take
-    // consecutive runs of whole chunks
+    // consecutive runs of whole chunks.  Every vector goes through the ring; what is outside the row is
+    // -inf there, so that it has probability 0
     const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-    const int64_t n_vec = ((int64_t)p.vocab + shift + VEC - 1) / VEC;
-    const int64_t chunks = (n_vec + kThreads * U - 1) / (kThreads * U);
-    const int64_t c0 = chunks * part / parts, c1 = chunks * (part + 1) / parts;
+    const int64_t end = (int64_t)p.vocab + shift;
+    const int chunks = (int)((end + CHUNK - 1) / CHUNK), inner0 = shift ? 1 : 0, inner1 = (int)(end / CHUNK);
+    const int c0 = (int)((int64_t)chunks * part / parts), c1 = (int)((int64_t)chunks * (part + 1) / parts);
 
-    if (tid == 0) s.count = 0;
-    __syncthreads();
-
-    auto load = [&](int64_t chunk, float (&v)[kElems]) {
+    const uint4* vectors = reinterpret_cast<const uint4*>(x - shift) + tid;
+    const uint32_t slots = smem_u32(ring) + tid * 16;
+    auto copy = [&](uint32_t dst, const uint4* src) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    };
+    auto load = [&](int chunk) {  // chunks behind the last are not read
+        const uint32_t dst = slots + (chunk - c0) % S * (U * kThreads * 16);
+        const uint4* src = vectors + (int64_t)chunk * (U * kThreads);
+        if (chunk >= inner0 && chunk < min(inner1, c1)) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int64_t vec = (chunk * U + u) * kThreads + tid, e0 = vec * VEC - shift;
-            if (e0 >= 0 && e0 + VEC <= p.vocab) {
-                const uint4 w = __ldcs(reinterpret_cast<const uint4*>(x + e0));
-                const uint32_t r[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if constexpr (sizeof(T) == 4) {
-                        v[u * VEC + i] = __uint_as_float(r[i]);
-                    } else {
-                        const T* h = reinterpret_cast<const T*>(&r[i]);
-                        v[u * VEC + 2 * i] = to_f32(h[0]);
-                        v[u * VEC + 2 * i + 1] = to_f32(h[1]);
-                    }
+            for (int u = 0; u < U; u++) copy(dst + u * kThreads * 16, src + u * kThreads);
+        } else if (chunk < c1) {  // an end of the row
+#pragma unroll 1
+            for (int u = 0; u < U; u++) {
+                const int64_t e0 = (int64_t)chunk * CHUNK + (u * kThreads + tid) * VEC - shift;
+                if (e0 >= 0 && e0 + VEC <= p.vocab) {
+                    copy(dst + u * kThreads * 16, src + u * kThreads);
+                    continue;
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    const int64_t e = e0 + i;
-                    v[u * VEC + i] = e >= 0 && e < p.vocab ? to_f32(x[e]) : -INFINITY;
-                }
+                T* to = reinterpret_cast<T*>(ring + ((chunk - c0) % S * U + u) * (kThreads * 16) + tid * 16);
+                for (int i = 0; i < VEC; i++) to[i] = e0 + i >= 0 && e0 + i < p.vocab ? x[e0 + i] : static_cast<T>(-INFINITY);
             }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    // place in the row of element i of the E elements of thread t in a chunk
+    auto place = [&](int chunk, int t, int i) {
+        return (int64_t)chunk * CHUNK + (i / VEC) * (kThreads * VEC) + t * VEC + i % VEC - shift;
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; i++) load(c0 + i);
+    if (lane == 0) s.published[warp] = -INFINITY;
 
     State st = {-INFINITY, 0.f, 0.f};
+    float c = 0.f, delta = 0.f, scale = 1.f;  // of st.m: m log2 e rounded, what was cut off, and 2^-delta
+    unsigned long long mine = 0;               // lane i: the warp's i-th largest key
     float thr = -INFINITY;
-    float cur[kElems], nxt[kElems];
-    if (c0 < c1) load(c0, cur);
-    for (int64_t chunk = c0; chunk < c1; chunk++) {
-        if (chunk + 1 < c1) load(chunk + 1, nxt);
-        float mx = cur[0];
+    for (int chunk = c0; chunk < c1; chunk++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+        const uint32_t src = slots + (chunk - c0) % S * (U * kThreads * 16);
+        float mx = -INFINITY;
+        uint32_t r[U * 4];
 #pragma unroll
-        for (int i = 1; i < kElems; i++) mx = fmaxf(mx, cur[i]);
+        for (int u = 0; u < U; u++)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(r[4 * u]), "=r"(r[4 * u + 1]), "=r"(r[4 * u + 2]), "=r"(r[4 * u + 3])
+                         : "r"(src + u * kThreads * 16)
+                         : "memory");
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < E; i++) mx = fmaxf(mx, __uint_as_float(r[i]));
+        } else {
+            using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+            T2 top = reinterpret_cast<const T2&>(r[0]);
+#pragma unroll
+            for (int i = 1; i < E / 2; i++) top = __hmax2(top, reinterpret_cast<const T2&>(r[i]));
+            const float2 f = unpack2<T>(reinterpret_cast<const uint32_t&>(top));
+            mx = fmaxf(f.x, f.y);
+        }
+        auto pair = [&](int i) {  // elements i and i + 1, i even
+            if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+            else return unpack2<T>(r[i / 2]);
+        };
+        load(chunk + S - 1);
+
         if (mx > st.m) {
             const float d = st.m - mx, w = __expf(d);
             st.t = w == 0.f ? 0.f : w * (st.t + st.z * d);
             st.z *= w;
             st.m = mx;
+            c = mx * kLog2e;
+            delta = fmaf(mx, kLog2e, -c);
+            scale = ex2(-delta);
         }
-        const float ref = st.m == -INFINITY ? 0.f : st.m;
+        // y = (x - m) log2 e + delta in one multiply-add: delta is what rounding c cost
+        bool plain = fabsf(st.m) < 1e6f;
+        if (plain) {
+            const float2 l2e = make_float2(kLog2e, kLog2e), off = make_float2(-c, -c);
+            float2 z = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < kElems; i++) {
-            const float d = cur[i] - ref, e = __expf(d);
-            st.z += e;
-            st.t += e * fmaxf(d, -1000.f);  // e is 0 there; -inf would make 0 * inf
+            for (int i = 0; i < E; i += 2) {
+                const float2 y = fma2(pair(i), l2e, off), e = make_float2(ex2(y.x), ex2(y.y));
+                z = add2(z, e);
+                t = fma2(e, y, t);
+            }
+            const float zs = z.x + z.y, ts = t.x + t.y;
+            plain = ts == ts;  // 0 * -inf where a logit is -inf
+            if (plain) {
+                st.z += scale * zs;
+                st.t += scale * kLn2 * (ts - delta * zs);
+            }
+        }
+        if (!plain) {  // an end of the row, a logit of -inf or NaN, a huge maximum
+            const float ref = st.m == -INFINITY ? 0.f : st.m;
+#pragma unroll
+            for (int i = 0; i < E; i += 2) {
+                const float2 f = pair(i);
+                const float d0 = max_nan(f.x - ref, -1000.f), d1 = max_nan(f.y - ref, -1000.f);  // e^-1000 is 0
+                const float e0 = ex2(d0 * kLog2e), e1 = ex2(d1 * kLog2e);
+                st.z += e0 + e1;
+                st.t += e0 * d0 + e1 * d1;
+            }
         }
         if (n > 0) {
-            const bool first = chunk == c0;
-            if (first) {  // the n-th largest of the maxima of 32 groups of 8 threads
+            if (chunk == c0) {
                 float g = mx;
 #pragma unroll
                 for (int o = 4; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
                 if ((tid & 7) == 0) s.group_max[tid >> 3] = ordered(g);
                 __syncthreads();
                 if (tid < 32) {
-                    const uint32_t mine = s.group_max[tid];
+                    const uint32_t me = s.group_max[tid];
                     int rank = 0;
-                    for (int i = 0; i < 32; i++) rank += s.group_max[i] > mine || (s.group_max[i] == mine && i < tid);
-                    if (rank == n - 1) s.threshold = unordered(mine);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) rank += s.group_max[i] > me || (s.group_max[i] == me && i < tid);
+                    if (rank == n - 1) s.first_threshold = unordered(me);
                 }
                 __syncthreads();
-                thr = s.threshold;
+                thr = s.first_threshold;
             }
-            bool full = false;
-#pragma unroll
-            for (int i = 0; i < kElems; i++) {
-                // later chunks hold higher indices only: an equal element loses there
-                if (first ? !(cur[i] < thr) : !(cur[i] <= thr)) {
-                    const int u = i / VEC;
-                    const int64_t e = ((chunk * U + u) * kThreads + tid) * VEC - shift + i % VEC;
-                    if (e >= 0 && e < p.vocab) {
-                        const int at = atomicAdd(&s.count, 1);
-                        s.key[at] = ((unsigned long long)ordered(cur[i]) << 32) | (uint32_t)~(uint32_t)e;
-                        full |= at >= kLimit;
+            // lanes with an element to look at (a maximum skips NaN, which counts as largest here: the sum shows it)
+            uint32_t look = __ballot_sync(0xffffffffu, !(mx < thr) || st.z != st.z);
+            const bool found = look != 0;
+            if (found) {
+                __syncwarp();  // the other lanes' copies
+                unsigned long long last = __shfl_sync(0xffffffffu, mine, n - 1);
+                for (; look; look &= look - 1) {
+                    const int t = warp * 32 + __ffs(look) - 1;
+                    // lane i takes element i of that lane
+                    const int64_t e = place(chunk, t, lane);
+                    unsigned long long key = 0;
+                    if (lane < E && e >= 0 && e < p.vocab) {
+                        const float v = to_f32(*reinterpret_cast<const T*>(
+                            ring + ((chunk - c0) % S * U + lane / VEC) * (kThreads * 16) + t * 16 + lane % VEC * sizeof(T)));
+                        if (!(v < thr)) key = ((unsigned long long)ordered(v) << 32) | (uint32_t)~(uint32_t)e;
+                    }
+                    uint32_t todo = __ballot_sync(0xffffffffu, key > last);
+                    while (todo) {
+                        const int from = __ffs(todo) - 1;
+                        const unsigned long long k = __shfl_sync(0xffffffffu, key, from);
+                        const int at = __popc(__ballot_sync(0xffffffffu, mine > k));
+                        const unsigned long long up = __shfl_up_sync(0xffffffffu, mine, 1);
+                        if (lane >= at) mine = lane == at ? k : up;
+                        last = __shfl_sync(0xffffffffu, mine, n - 1);
+                        todo &= __ballot_sync(0xffffffffu, key > last) & ~(1u << from);
                     }
                 }
+                if (last) thr = fmaxf(thr, unordered((uint32_t)(last >> 32)));
+                const unsigned long long share = __shfl_sync(0xffffffffu, mine, (n - 1) / kWarps);
+                if (lane == 0 && share) s.published[warp] = unordered((uint32_t)(share >> 32));
             }
-            if (__syncthreads_or(full)) {
-                const int kept = keep_largest(s, s.count, n);
-                if (tid == 0) s.count = kept;
-                if (kept == n) thr = unordered((uint32_t)(s.key[n - 1] >> 32));
-                __syncthreads();
+            if (found || chunk % 4 == 0) {
+                float shared = s.published[lane % kWarps];
+#pragma unroll
+                for (int o = 1; o < kWarps; o <<= 1) shared = fminf(shared, __shfl_xor_sync(0xffffffffu, shared, o));
+                thr = fmaxf(thr, shared);
             }
         }
-#pragma unroll
-        for (int i = 0; i < kElems; i++) cur[i] = nxt[i];
     }
 
-    // the CTA's state, in a fixed order
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const State other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.z, o),
-                             __shfl_xor_sync(0xffffffffu, st.t, o)};
-        st = (tid & o) ? join(other, st) : join(st, other);
-    }
-    if ((tid & 31) == 0) s.warp_state[tid >> 5] = st;
+    // the CTA's state and list
+    st = join_lanes(st, 32);
+    if (lane == 0) s.warp_state[warp] = st;
+    s.list[warp][lane] = lane < n ? mine : 0;
     __syncthreads();
-    int count = s.count;
-    if (n > 0) count = keep_largest(s, count, n);
-    if (tid == 0) {
-        st = s.warp_state[0];
-        for (int w = 1; w < kThreads / 32; w++) st = join(st, s.warp_state[w]);
-        s.state = st;
-        s.count = count;
+    merge_lists(s.list, kWarps, n, s.largest);
+    if (warp == 0) {
+        st = join_lanes(s.warp_state[lane % kWarps], kWarps);
+        if (lane == 0) s.state = st;
     }
     if (parts > 1) {
         cluster_sync();  // every part's state and list are complete
         if (part == 0) {
-            // the other parts' lists behind this one's, then the n largest of all
-            int total = count;
-            for (int q = 1; q < parts; q++) {
-                const int c = n > 0 ? ld_peer_s32(mapa(smem_u32(&s.count), q)) : 0;
-                if (tid < c) s.key[total + tid] = ld_peer_u64(mapa(smem_u32(&s.key[tid]), q));
-                total += c;
+            if (warp < parts) s.list[warp][lane] = lane < n ? ld_peer_u64(mapa(smem_u32(&s.largest[lane]), warp)) : 0;
+            if (warp == 0) {
+                const int q = lane & (parts - 1);
+                st = {ld_peer_f32(mapa(smem_u32(&s.state.m), q)), ld_peer_f32(mapa(smem_u32(&s.state.z), q)),
+                      ld_peer_f32(mapa(smem_u32(&s.state.t), q))};
+                st = join_lanes(st, parts);
             }
-            if (tid == 0) {
-                for (int q = 1; q < parts; q++) {
-                    const State other = {ld_peer_f32(mapa(smem_u32(&s.state.m), q)),
-                                         ld_peer_f32(mapa(smem_u32(&s.state.z), q)),
-                                         ld_peer_f32(mapa(smem_u32(&s.state.t), q))};
-                    st = join(st, other);
-                }
-                s.state = st;
-            }
-            __syncthreads();
-            if (n > 0) count = keep_largest(s, total, n);
         }
-        cluster_sync();  // nobody leaves while its shared memory is read
+        cluster_sync();  // nobody leaves, or is overwritten, while its shared memory is read
         if (part != 0) return;
-    } else {
-        __syncthreads();
+        if (tid == 0) s.state = st;
+        merge_lists(s.list, parts, n, s.largest);
     }
+    __syncthreads();
     const State all = s.state;
     const float log_z = logf(all.z);
     if (tid < n) {
-        const unsigned long long k = s.key[tid];
+        const unsigned long long k = s.largest[tid];
         p.top_id[(int64_t)row * n + tid] = (int32_t) ~(uint32_t)k;
         p.top_logprob[(int64_t)row * n + tid] = (unordered((uint32_t)(k >> 32)) - all.m) - log_z;
     }
@@ -325,7 +380,7 @@ cudaError_t launch_t(const LogprobParams& p, int parts, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((int64_t)p.rows * parts));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = sizeof(Shared);
+    cfg.dynamicSmemBytes = kRing;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -339,18 +394,19 @@ cudaError_t launch_t(const LogprobParams& p, int parts, cudaStream_t st) {
 }  // namespace
 
 cudaError_t logprobs_init_device() {
-    cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+    cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(logprobs_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+        e = cudaFuncSetAttribute(logprobs_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(logprobs_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+        e = cudaFuncSetAttribute(logprobs_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
     return e;
 }
 
 cudaError_t launch_logprobs(int type, const LogprobParams& p, int sms, cudaStream_t st) {
     // CTAs per row: as many as fit the GPU twice over, while each still has two chunks
+    const int chunk = kThreads * kVecs * (type == TPTC_TYPE_F32 ? 4 : 8);
     int parts = 1;
-    while (parts < 8 && (int64_t)p.rows * parts * 2 <= 2 * sms && p.vocab / (parts * 2) >= 2 * kChunk) parts *= 2;
+    while (parts < kMaxParts && (int64_t)p.rows * parts * 2 <= 2 * sms && p.vocab / (parts * 2) >= 2 * chunk) parts *= 2;
     if (type == TPTC_TYPE_F16) return launch_t<__half>(p, parts, st);
     if (type == TPTC_TYPE_BF16) return launch_t<__nv_bfloat16>(p, parts, st);
     return launch_t<float>(p, parts, st);
