@@ -29,8 +29,8 @@ namespace {
 constexpr int BM = 128, BN = 128;
 constexpr int kThreads = 384;  // warpgroup 0: copies (warp 0) and products (warp 1); 1 and 2: the softmax of A and B
 // Registers: 384 threads launch with 168 each; the softmax threads hold 128 scores and take what
-// warpgroup 0 gives back (128 x (56 + 2 x 216) <= 384 x 168).
-constexpr int kRegsFew = 56, kRegsMany = 216;
+// warpgroup 0 gives back (128 x (72 + 2 x 216) = 384 x 168).
+constexpr int kRegsFew = 72, kRegsMany = 216;
 constexpr int kTmemCols = 512;
 
 template <int HD>
@@ -65,6 +65,14 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, u
         " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
         "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)
         : "memory");
+}
+
+// One lane of a converged warp.  (The compiler keeps what a warp computes alike in uniform registers, where
+// the products' operands have to be; under `lane == 0` each product cost about 100 cycles to issue.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(one));
+    return one != 0;
 }
 
 // 32 columns, not waited for; tmem_loaded() below ends the wait for all loads before it.
@@ -128,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int S = L::kStages, KS = HD / 16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t q_full, full[S], empty[S], s_full[2], p_full[2], o_done[2], drain;
+    __shared__ uint64_t q_full, full[S], empty[S], s_full[2], p_full[2][2], o_done[2], drain;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -160,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int t = 0; t < 2; t++) {
             mbar_init(&s_full[t], 1);
-            mbar_init(&p_full[t], 4);  // one arrival per softmax warp
+            for (int h = 0; h < 2; h++) mbar_init(&p_full[t][h], 4);  // one arrival per softmax warp
             mbar_init(&o_done[t], 1);
         }
         mbar_init(&drain, 1);
@@ -199,52 +207,72 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_wait_bounded(&q_full, 0, nullptr);
             for (int k = i > S ? i - S : 0; k < i; k++) mbar_wait_bounded(&full[k % S], (k / S) & 1, nullptr);
         }
-        if (warp == 1 && lane == 0 && ntot > 0) {  // products
+        if (warp == 1 && ntot > 0) {  // products: the whole warp waits, one elected lane issues
             constexpr uint32_t type_bits = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
-            const uint32_t id_s = mma_idesc(BM, BN) | type_bits, id_o = mma_idesc(BM, HD) | kIdescBMajorMN | type_bits;
-            auto slot = [&](int i) { return smem_u32(smem + L::kKV + (i % S) * L::kTileBytes); };
-            auto wait_full = [&](int i) { return wait_or_abort(&full[i % S], (i / S) & 1, p.status, &abort_flag); };
+            constexpr uint32_t id_s = mma_idesc(BM, BN) | type_bits, id_o = mma_idesc(BM, HD) | kIdescBMajorMN | type_bits;
+            // (descriptors hold the address / 16 in their low bits: steps inside a tile are added there)
+            const uint64_t q_desc = sw128_desc(smem_u32(smem)), k_desc = sw128_desc(smem_u32(smem + L::kKV));
+            const uint64_t v_desc = sw128_desc_mn(smem_u32(smem + L::kKV), BN * 128);
+            const bool one = elect_one();
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                return __all_sync(0xffffffffu, wait_or_abort(bar, parity, p.status, &abort_flag)) != 0;
+            };
+            auto wait_full = [&](int i) { return wait(&full[i % S], (i / S) & 1); };
             auto issue_s = [&](int t, int j) {
-                const uint32_t qa = smem_u32(smem + t * L::kTileBytes), ka = slot(2 * j);
+                const uint64_t qa = q_desc + t * (L::kTileBytes / 16), ka = k_desc + (2 * j) % S * (L::kTileBytes / 16);
+                if (one) {
 #pragma unroll
-                for (int k = 0; k < KS; k++)
-                    mma_f16(tmem + BN * t, sw128_desc(qa + (k / 4) * BM * 128 + 32 * (k % 4)),
-                            sw128_desc(ka + (k / 4) * BN * 128 + 32 * (k % 4)), id_s, k != 0);
-                mma_commit(&s_full[t]);
+                    for (int k = 0; k < KS; k++) {
+                        const int at = ((k / 4) * BN * 128 + 32 * (k % 4)) / 16;
+                        mma_f16(tmem + BN * t, qa + at, ka + at, id_s, k != 0);
+                    }
+                    mma_commit(&s_full[t]);
+                }
             };
-            auto issue_pv = [&](int t, int j) {
-                const uint32_t va = slot(2 * j + 1);
+            auto issue_pv = [&](int t, int j, int half) {
+                const uint64_t va = v_desc + (2 * j + 1) % S * (L::kTileBytes / 16);
+                if (one) {
 #pragma unroll
-                for (int k = 0; k < BN / 16; k++)
-                    mma_ts(tmem + 256 + 128 * t, tmem + BN * t + 8 * k, sw128_desc_mn(va + k * 2048, BN * 128), id_o, (j | k) != 0);
+                    for (int k = half * (BN / 32); k < (half + 1) * (BN / 32); k++)
+                        mma_ts(tmem + 256 + 128 * t, tmem + BN * t + 8 * k, va + k * (2048 / 16), id_o, (j | k) != 0);
+                }
             };
-            bool ok = wait_or_abort(&q_full, 0, p.status, &abort_flag) && wait_full(0);
+            auto commit = [&](uint64_t* bar) {
+                if (one) mma_commit(bar);
+            };
+            bool ok = wait(&q_full, 0) && wait_full(0);
             if (ok) {
                 tc_fence_after();
                 for (int t = 0; t < 2; t++)
                     if (nt[t] > 0) issue_s(t, 0);
-                mma_commit(&empty[0]);
+                commit(&empty[0]);
             }
             for (int j = 0; j < ntot && ok; j++) {
                 const bool more = j + 1 < ntot;
                 ok = wait_full(2 * j + 1) && (!more || wait_full(2 * j + 2));
                 for (int t = 0; t < 2 && ok; t++) {
                     if (j >= nt[t]) continue;
-                    ok = wait_or_abort(&p_full[t], j & 1, p.status, &abort_flag);
+                    // the weights come in two halves
+                    ok = wait(&p_full[t][0], j & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    issue_pv(t, j);
+                    issue_pv(t, j, 0);
+                    ok = wait(&p_full[t][1], j & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_pv(t, j, 1);
                     if (j + 1 < nt[t]) issue_s(t, j + 1);
-                    else mma_commit(&o_done[t]);
+                    else commit(&o_done[t]);
                 }
                 if (ok) {  // V_j and K_(j + 1) are used up
-                    mma_commit(&empty[(2 * j + 1) % S]);
-                    if (more) mma_commit(&empty[(2 * j + 2) % S]);
+                    commit(&empty[(2 * j + 1) % S]);
+                    if (more) commit(&empty[(2 * j + 2) % S]);
                 }
             }
             // every product issued has completed before TMEM is freed
-            mma_commit(&drain);
+            commit(&drain);
             mbar_wait_bounded(&drain, 0, nullptr);
+            __syncwarp();
         }
     } else {  // one thread per lane of tile A or B
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
@@ -295,23 +323,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_st32_async(tO + c, w);
                 }
             }
-            const float neg = m == -INFINITY ? 0.f : -m;  // a lane that sees nothing yet: weights 0
-            const float2 sc = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
-            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-            for (int c = 0; c < BN; c += 64) {
-                uint32_t w[32];
-#pragma unroll
-                for (int k = 0; k < 32; k++) {
-                    const float2 y = fma2(make_float2(s[c + 2 * k], s[c + 2 * k + 1]), sc, off);
-                    const float2 e = make_float2(ex2(y.x), ex2(y.y));
-                    sum[k & 1] = add2(sum[k & 1], e);
-                    w[k] = pack2<T>(e.x, e.y);
-                }
-                tmem_st32_async(tS + c / 2, w);
-            }
-            sum[0] = add2(sum[0], sum[1]);
-            l += sum[0].x + sum[0].y;
             if ((j + 1) * BN > lk &&
                 __all_sync(0xffffffffu, wait_or_abort(&full[(2 * j + 1) % S], ((2 * j + 1) / S) & 1, p.status, &abort_flag))) {
                 // rows behind the sequence's last key may hold anything: zero them in V, so that
@@ -324,10 +335,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 fence_proxy_async_smem();
             }
-            tmem_stores_done();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
+            const float neg = m == -INFINITY ? 0.f : -m;  // a lane that sees nothing yet: weights 0
+            const float2 sc = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t w[32];
+#pragma unroll
+                for (int k = 0; k < 32; k++) {
+                    const float2 y = fma2(make_float2(s[64 * h + 2 * k], s[64 * h + 2 * k + 1]), sc, off);
+                    const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                    sum[k & 1] = add2(sum[k & 1], e);
+                    w[k] = pack2<T>(e.x, e.y);
+                }
+                tmem_st32_async(tS + 32 * h, w);
+                tmem_stores_done();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t][h]);
+            }
+            sum[0] = add2(sum[0], sum[1]);
+            l += sum[0].x + sum[0].y;
         }
         if (ok && nt[t] > 0) ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[t], 0, p.status, &abort_flag));
         if (ok && toks[t] > 0) {
