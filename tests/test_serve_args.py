@@ -100,7 +100,7 @@ def packed(**kw):
     (UNSUPPORTED, dict(type_=K.F32)), (UNSUPPORTED, dict(head_dim=256)), (UNSUPPORTED, dict(n_heads=258, q_stride=1 << 20)),
     (ARG, dict(n_heads=3)), (ARG, dict(n_kv=0)), (ARG, dict(n_heads=0)), (ARG, dict(n_seq=-1)), (ARG, dict(n_q=-1)),
     (ARG, dict(n_k=-1)), (ARG, dict(max_q=-1)), (ARG, dict(n_k=2 ** 31 - 100)), (ARG, dict(d_q=0)), (ARG, dict(d_cu_k=0)),
-    (ARG, dict(d_out=P + 8)), (ARG, dict(q_stride=248)), (ARG, dict(k_stride=130)), (ARG, dict(d_v=P + 2))])
+    (ARG, dict(d_out=P + 16)), (ARG, dict(q_stride=248)), (ARG, dict(k_stride=130)), (ARG, dict(d_v=P + 2))])
 def test_prompts(code, kw):
     refused(code, packed, **kw)
 

@@ -45,7 +45,8 @@ struct Lay {
 struct Params {
     void* out;
     const int32_t *cu_q, *cu_k;
-    int n_seq, n_q, n_k, max_q, n_heads, n_kv, tokens;  // tokens per tile
+    int n_seq, n_q, n_k, max_q, n_heads, n_kv;
+    int tokens, pairs;  // tokens per tile; pairs of tiles of the longest sequence
     float scale_log2;
     int32_t* status;
 };
@@ -111,6 +112,12 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 32 bytes of a row (a whole sector) in one store.
+__device__ __forceinline__ void store32(void* p, const uint32_t* r) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 // Two f32 fused multiply-adds or sums in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;
@@ -128,6 +135,63 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+// ---- work items.  A CTA that is through with its own block index takes over that of a CTA that has not
+// started yet (cluster launch control), so that TMEM, barriers and the ring are set up once per SM, the next
+// item's loads run under the current one's last products, and the hardware balances ragged batches.
+
+__device__ __forceinline__ void request_item(uint4* response, uint64_t* bar) {
+    mbar_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(response)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// The block index taken over, or -1 when none was left.
+__device__ __forceinline__ int taken_item(const uint4* response) {
+    uint32_t x, got;
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b128 r;\n ld.shared.b128 r, [%2];\n"
+        " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.u32 %1, 1, 0, p;\n mov.u32 %0, 0;\n"
+        " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, r;\n}\n"
+        : "=&r"(x), "=&r"(got)
+        : "r"(smem_u32(response))
+        : "memory");
+    return got ? (int)x : -1;
+}
+
+struct Item {
+    int q0, k0;     // packed rows: the first token of tile A, the sequence's first key
+    int kvh;
+    int base, lk;   // tile A's first token sees base + 1 keys; keys of the sequence
+    int toks[2], nt[2], ntot;  // tokens of a tile, and the key tiles that its last token sees
+};
+// Every role decodes an item for itself, alike; false: nothing to do.
+__device__ __forceinline__ bool decode(const Params& p, int index, Item& w) {
+    // the pairs of tiles with the most keys first
+    const int per = p.n_kv * p.n_seq, pair = p.pairs - 1 - index / per, at = index % per, b = at / p.n_kv;
+    w.kvh = at % p.n_kv;
+    const int q_lo = p.cu_q[b], q_hi = p.cu_q[b + 1], k_lo = p.cu_k[b], k_hi = p.cu_k[b + 1];
+    if (q_lo == q_hi) return false;
+    if (q_lo < 0 || q_hi < q_lo || q_hi > p.n_q || q_hi - q_lo > p.max_q || k_lo < 0 || k_hi < k_lo || k_hi > p.n_k) {
+        if (pair == 0 && threadIdx.x == 0 && p.status) atomicExch(p.status, TPTC_ERR_ARG);
+        return false;
+    }
+    const int lq = q_hi - q_lo, lk = k_hi - k_lo, tok0 = pair * 2 * p.tokens;
+    if (tok0 >= lq) return false;
+    w.q0 = q_lo + tok0;
+    w.k0 = k_lo;
+    w.lk = lk;
+    w.base = lk - lq + tok0;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        w.toks[t] = max(0, min(p.tokens, lq - tok0 - t * p.tokens));
+        const int sees = w.base + t * p.tokens + w.toks[t];
+        w.nt[t] = w.toks[t] > 0 && sees > 0 ? (sees + BN - 1) / BN : 0;
+    }
+    w.ntot = max(w.nt[0], w.nt[1]);
+    return true;
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_packed_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -136,32 +200,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int S = L::kStages, KS = HD / 16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t q_full, full[S], empty[S], s_full[2], p_full[2][2], o_done[2], drain;
+    __shared__ uint64_t q_full, q_empty, full[S], empty[S], s_full[2], p_full[2][2], o_done[2], drain, item_full[2], item_empty[2];
+    __shared__ uint4 response[2];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = p.n_heads / p.n_kv;
-    // the pairs of tiles with the most keys first
-    const int per = p.n_kv * p.n_seq, pairs = gridDim.x / per;
-    const int pair = pairs - 1 - blockIdx.x / per, kvh = blockIdx.x % per % p.n_kv, b = blockIdx.x % per / p.n_kv;
-    const int q_lo = p.cu_q[b], q_hi = p.cu_q[b + 1], k_lo = p.cu_k[b], k_hi = p.cu_k[b + 1];
-    if (q_lo == q_hi) return;
-    if (q_lo < 0 || q_hi < q_lo || q_hi > p.n_q || q_hi - q_lo > p.max_q || k_lo < 0 || k_hi < k_lo || k_hi > p.n_k) {
-        if (pair == 0 && threadIdx.x == 0 && p.status) atomicExch(p.status, TPTC_ERR_ARG);
-        return;
-    }
-    const int lq = q_hi - q_lo, lk = k_hi - k_lo, tok0 = pair * 2 * p.tokens;
-    if (tok0 >= lq) return;
-    int toks[2], nt[2];  // tokens of a tile, and the key tiles that its last token sees
-    for (int t = 0; t < 2; t++) {
-        toks[t] = max(0, min(p.tokens, lq - tok0 - t * p.tokens));
-        const int sees = lk - lq + tok0 + t * p.tokens + toks[t];
-        nt[t] = toks[t] > 0 && sees > 0 ? (sees + BN - 1) / BN : 0;
-    }
-    const int ntot = max(nt[0], nt[1]);
 
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
+        mbar_init(&q_empty, 1);
         for (int s = 0; s < S; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
@@ -170,6 +218,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&s_full[t], 1);
             for (int h = 0; h < 2; h++) mbar_init(&p_full[t][h], 4);  // one arrival per softmax warp
             mbar_init(&o_done[t], 1);
+            mbar_init(&item_full[t], 1);
+            mbar_init(&item_empty[t], 9);  // the product warp and eight softmax warps have read it
         }
         mbar_init(&drain, 1);
         fence_mbar_init();
@@ -180,34 +230,63 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    // the next item's index for a warp of the products or the softmax, which has had n of them (-1: no more)
+    auto next_item = [&](int n) {
+        const int s = (n - 1) & 1;
+        if (!__all_sync(0xffffffffu, wait_or_abort(&item_full[s], ((n - 1) >> 1) & 1, p.status, &abort_flag))) return -1;
+        const int index = taken_item(&response[s]);
+        fence_proxy_async_smem();  // read before the slot is written again
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[s]);
+        return index;
+    };
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
-        if (warp == 0 && lane == 0 && ntot > 0) {  // copies: Q_A, Q_B, then K_0, V_0, K_1, ...
-            const uint32_t q_bytes = (uint32_t)(p.tokens * G) * 128 * L::NC;
-            mbar_expect_tx(&q_full, (toks[1] > 0 ? 2 : 1) * q_bytes);
-            for (int t = 0; t < 2; t++) {
-                if (toks[t] == 0) continue;
+        if (warp == 0 && lane == 0) {  // copies: Q_A, Q_B, then K_0, V_0, K_1, ... of each item
+            int i0 = 0, nq = 0;        // loads into the ring and Q tiles so far
+            bool ok = true;
+            int index = blockIdx.x;
+            for (int n = 1; ok; n++) {
+                Item w;
+                if (decode(p, index, w) && w.ntot > 0) {
+                    if (nq > 0) ok = wait_or_abort(&q_empty, (nq - 1) & 1, p.status, &abort_flag);
+                    if (!ok) break;
+                    nq++;
+                    mbar_expect_tx(&q_full, (w.toks[1] > 0 ? 2 : 1) * ((uint32_t)(p.tokens * G) * 128 * L::NC));
+                    for (int t = 0; t < 2; t++) {
+                        if (w.toks[t] == 0) continue;
 #pragma unroll
-                for (int c = 0; c < L::NC; c++)
-                    tma_load_3d(smem + t * L::kTileBytes + c * BM * 128, &tq, c * 64, kvh * G, q_lo + tok0 + t * p.tokens,
-                                &q_full);
-            }
-            int i = 0;
-            for (; i < 2 * ntot; i++) {
-                const int s = i % S;
-                if (i >= S && !wait_or_abort(&empty[s], ((i / S) - 1) & 1, p.status, &abort_flag)) break;
-                mbar_expect_tx(&full[s], L::kTileBytes);
+                        for (int c = 0; c < L::NC; c++)
+                            tma_load_3d(smem + t * L::kTileBytes + c * BM * 128, &tq, c * 64, w.kvh * G, w.q0 + t * p.tokens,
+                                        &q_full);
+                    }
+                    for (int k = 0; k < 2 * w.ntot; k++, i0++) {
+                        const int s = i0 % S;
+                        if (i0 >= S) ok = wait_or_abort(&empty[s], ((i0 / S) - 1) & 1, p.status, &abort_flag);
+                        if (!ok) break;
+                        mbar_expect_tx(&full[s], L::kTileBytes);
 #pragma unroll
-                for (int c = 0; c < L::NC; c++)
-                    tma_load_3d(smem + L::kKV + s * L::kTileBytes + c * BN * 128, (i & 1) ? &tv : &tk, c * 64, kvh,
-                                k_lo + (i >> 1) * BN, &full[s]);
+                        for (int c = 0; c < L::NC; c++)
+                            tma_load_3d(smem + L::kKV + s * L::kTileBytes + c * BN * 128, (k & 1) ? &tv : &tk, c * 64, w.kvh,
+                                        w.k0 + (k >> 1) * BN, &full[s]);
+                    }
+                    if (!ok) break;
+                }
+                const int s = (n - 1) & 1;
+                if (n > 2) ok = wait_or_abort(&item_empty[s], ((n - 3) >> 1) & 1, p.status, &abort_flag);
+                if (!ok) break;
+                request_item(&response[s], &item_full[s]);
+                ok = wait_or_abort(&item_full[s], ((n - 1) >> 1) & 1, p.status, &abort_flag);
+                if (!ok) break;
+                index = taken_item(&response[s]);
+                if (index < 0) break;
             }
             // the copies still in flight land before the CTA exits
-            mbar_wait_bounded(&q_full, 0, nullptr);
-            for (int k = i > S ? i - S : 0; k < i; k++) mbar_wait_bounded(&full[k % S], (k / S) & 1, nullptr);
+            if (nq > 0) mbar_wait_bounded(&q_full, (nq - 1) & 1, nullptr);
+            for (int k = i0 > S ? i0 - S : 0; k < i0; k++) mbar_wait_bounded(&full[k % S], (k / S) & 1, nullptr);
         }
-        if (warp == 1 && ntot > 0) {  // products: the whole warp waits, one elected lane issues
+        if (warp == 1) {  // products: the whole warp waits, one elected lane issues
             constexpr uint32_t type_bits = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
             constexpr uint32_t id_s = mma_idesc(BM, BN) | type_bits, id_o = mma_idesc(BM, HD) | kIdescBMajorMN | type_bits;
             // (descriptors hold the address / 16 in their low bits: steps inside a tile are added there)
@@ -218,8 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 return __all_sync(0xffffffffu, wait_or_abort(bar, parity, p.status, &abort_flag)) != 0;
             };
             auto wait_full = [&](int i) { return wait(&full[i % S], (i / S) & 1); };
-            auto issue_s = [&](int t, int j) {
-                const uint64_t qa = q_desc + t * (L::kTileBytes / 16), ka = k_desc + (2 * j) % S * (L::kTileBytes / 16);
+            auto issue_s = [&](int t, int i) {  // i: the load of K
+                const uint64_t qa = q_desc + t * (L::kTileBytes / 16), ka = k_desc + i % S * (L::kTileBytes / 16);
                 if (one) {
 #pragma unroll
                     for (int k = 0; k < KS; k++) {
@@ -229,45 +308,60 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mma_commit(&s_full[t]);
                 }
             };
-            auto issue_pv = [&](int t, int j, int half) {
-                const uint64_t va = v_desc + (2 * j + 1) % S * (L::kTileBytes / 16);
+            auto issue_pv = [&](int t, int i, bool first, int half) {  // i: the load of V
+                const uint64_t va = v_desc + i % S * (L::kTileBytes / 16);
                 if (one) {
 #pragma unroll
                     for (int k = half * (BN / 32); k < (half + 1) * (BN / 32); k++)
-                        mma_ts(tmem + 256 + 128 * t, tmem + BN * t + 8 * k, va + k * (2048 / 16), id_o, (j | k) != 0);
+                        mma_ts(tmem + 256 + 128 * t, tmem + BN * t + 8 * k, va + k * (2048 / 16), id_o, !first || k != 0);
                 }
             };
             auto commit = [&](uint64_t* bar) {
                 if (one) mma_commit(bar);
             };
-            bool ok = wait(&q_full, 0) && wait_full(0);
-            if (ok) {
-                tc_fence_after();
-                for (int t = 0; t < 2; t++)
-                    if (nt[t] > 0) issue_s(t, 0);
-                commit(&empty[0]);
-            }
-            for (int j = 0; j < ntot && ok; j++) {
-                const bool more = j + 1 < ntot;
-                ok = wait_full(2 * j + 1) && (!more || wait_full(2 * j + 2));
-                for (int t = 0; t < 2 && ok; t++) {
-                    if (j >= nt[t]) continue;
-                    // the weights come in two halves
-                    ok = wait(&p_full[t][0], j & 1);
+            int i0 = 0, nq = 0, np[2] = {0, 0};  // loads, Q tiles and weight tiles before this item
+            bool ok = true;
+            int index = blockIdx.x;
+            for (int n = 1; index >= 0; n++) {
+                Item w;
+                if (decode(p, index, w) && w.ntot > 0) {
+                    ok = wait(&q_full, nq & 1) && wait_full(i0);
                     if (!ok) break;
+                    nq++;
                     tc_fence_after();
-                    issue_pv(t, j, 0);
-                    ok = wait(&p_full[t][1], j & 1);
+                    for (int t = 0; t < 2; t++)
+                        if (w.nt[t] > 0) issue_s(t, i0);
+                    commit(&empty[i0 % S]);
+                    if (w.ntot == 1) commit(&q_empty);
+                    for (int j = 0; j < w.ntot && ok; j++) {
+                        const bool more = j + 1 < w.ntot;
+                        const int iv = i0 + 2 * j + 1, ik = iv + 1;
+                        ok = wait_full(iv) && (!more || wait_full(ik));
+                        for (int t = 0; t < 2 && ok; t++) {
+                            if (j >= w.nt[t]) continue;
+                            // the weights come in two halves
+                            ok = wait(&p_full[t][0], np[t] & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            issue_pv(t, iv, j == 0, 0);
+                            ok = wait(&p_full[t][1], np[t] & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            issue_pv(t, iv, j == 0, 1);
+                            np[t]++;
+                            if (j + 1 < w.nt[t]) issue_s(t, ik);
+                            else commit(&o_done[t]);
+                        }
+                        if (ok) {  // V_j and K_(j + 1) are used up; Q with the last of them
+                            commit(&empty[iv % S]);
+                            if (more) commit(&empty[ik % S]);
+                            if (j + 2 == w.ntot) commit(&q_empty);
+                        }
+                    }
                     if (!ok) break;
-                    tc_fence_after();
-                    issue_pv(t, j, 1);
-                    if (j + 1 < nt[t]) issue_s(t, j + 1);
-                    else commit(&o_done[t]);
+                    i0 += 2 * w.ntot;
                 }
-                if (ok) {  // V_j and K_(j + 1) are used up
-                    commit(&empty[(2 * j + 1) % S]);
-                    if (more) commit(&empty[(2 * j + 2) % S]);
-                }
+                index = next_item(n);
             }
             // every product issued has completed before TMEM is freed
             commit(&drain);
@@ -279,107 +373,122 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int t = (warp >> 2) - 1, r = 32 * (warp & 3) + lane;
         const uint32_t loff = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t tS = tmem + BN * t + loff, tO = tmem + 256 + 128 * t + loff;
-        const int tok = tok0 + t * p.tokens + min(r / G, max(toks[t] - 1, 0));  // spare lanes follow the last token
-        const int sees = lk - lq + tok + 1;                                  // keys of this lane
-        const int all_see = lk - lq + tok0 + t * p.tokens + 1;               // keys that every lane of the tile sees
-        float m = -INFINITY, l = 0.f;
+        int i0 = 0, ns = 0, no = 0;  // loads, score tiles and outputs before this item
         bool ok = true;
-        for (int j = 0; j < nt[t]; j++) {
-            ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[t], j & 1, p.status, &abort_flag));
-            if (!ok) break;
-            tc_fence_after();
-            float s[BN];
+        int index = blockIdx.x;
+        for (int n = 1; index >= 0; n++) {
+            Item w;
+            if (decode(p, index, w)) {
+                const int nt = t ? w.nt[1] : w.nt[0], toks = t ? w.toks[1] : w.toks[0];
+                const int tok = t * p.tokens + min(r / G, max(toks - 1, 0));  // spare lanes follow the last token
+                const int sees = w.base + tok + 1, all_see = w.base + t * p.tokens + 1;  // keys of this lane, and of every lane
+                float m = -INFINITY, l = 0.f;
+                for (int j = 0; j < nt; j++, ns++) {
+                    ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[t], ns & 1, p.status, &abort_flag));
+                    if (!ok) break;
+                    tc_fence_after();
+                    float s[BN];
 #pragma unroll
-            for (int c = 0; c < BN; c += 32) tmem_ld32_async(tS + c, s + c);
-            tmem_loads_done();
-#pragma unroll
-            for (int c = 0; c < BN; c += 32) pin32(s + c);
-            if ((j + 1) * BN > all_see) {
-                const int left = sees - j * BN;
-#pragma unroll
-                for (int k = 0; k < BN; k++) s[k] = k < left ? s[k] : -INFINITY;
-            }
-            float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int k = 4; k < BN; k++) mx[k & 3] = fmaxf(mx[k & 3], s[k]);
-            const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-            const bool move = mt > m + 8.f;
-            float alpha = 1.f;
-            if (move) {
-                alpha = ex2(m - mt);
-                l *= alpha;
-                m = mt;
-            }
-            if (j > 0 && __any_sync(0xffffffffu, move)) {
-#pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
-                    float o[32];
-                    uint32_t w[32];
-                    tmem_ld32_async(tO + c, o);
+                    for (int c = 0; c < BN; c += 32) tmem_ld32_async(tS + c, s + c);
                     tmem_loads_done();
-                    pin32(o);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) w[i] = __float_as_uint(o[i] * alpha);
-                    tmem_st32_async(tO + c, w);
-                }
-            }
-            if ((j + 1) * BN > lk &&
-                __all_sync(0xffffffffu, wait_or_abort(&full[(2 * j + 1) % S], ((2 * j + 1) / S) & 1, p.status, &abort_flag))) {
-                // rows behind the sequence's last key may hold anything: zero them in V, so that
-                // weight 0 times them is 0 (both tiles write the same zeros, each before its product)
-                uint8_t* vb = smem + L::kKV + ((2 * j + 1) % S) * L::kTileBytes;
-                const int r0 = lk - j * BN, n = (BN - r0) * L::NC * 8;
-                for (int i = r; i < n; i += BM) {
-                    const int row = r0 + i / (L::NC * 8), rem = i % (L::NC * 8);
-                    *reinterpret_cast<uint4*>(vb + (rem >> 3) * BN * 128 + row * 128 + (rem & 7) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async_smem();
-            }
-            const float neg = m == -INFINITY ? 0.f : -m;  // a lane that sees nothing yet: weights 0
-            const float2 sc = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
-            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    for (int c = 0; c < BN; c += 32) pin32(s + c);
+                    if ((j + 1) * BN > all_see) {
+                        const int left = sees - j * BN;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint32_t w[32];
+                        for (int k = 0; k < BN; k++) s[k] = k < left ? s[k] : -INFINITY;
+                    }
+                    float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int k = 0; k < 32; k++) {
-                    const float2 y = fma2(make_float2(s[64 * h + 2 * k], s[64 * h + 2 * k + 1]), sc, off);
-                    const float2 e = make_float2(ex2(y.x), ex2(y.y));
-                    sum[k & 1] = add2(sum[k & 1], e);
-                    w[k] = pack2<T>(e.x, e.y);
-                }
-                tmem_st32_async(tS + 32 * h, w);
-                tmem_stores_done();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[t][h]);
-            }
-            sum[0] = add2(sum[0], sum[1]);
-            l += sum[0].x + sum[0].y;
-        }
-        if (ok && nt[t] > 0) ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[t], 0, p.status, &abort_flag));
-        if (ok && toks[t] > 0) {
-            tc_fence_after();
-            const float il = l > 0.f || l != l ? 1.f / l : 0.f;
-            const bool mine = r < toks[t] * G;
-            T* row = static_cast<T*>(p.out) + ((int64_t)(q_lo + tok) * p.n_heads + kvh * G + r % G) * HD;
+                    for (int k = 4; k < BN; k++) mx[k & 3] = fmaxf(mx[k & 3], s[k]);
+                    const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                    const bool move = mt > m + 8.f;
+                    float alpha = 1.f;
+                    if (move) {
+                        alpha = ex2(m - mt);
+                        l *= alpha;
+                        m = mt;
+                    }
+                    if (j > 0 && __any_sync(0xffffffffu, move)) {
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-                float o[32];
-                if (nt[t] > 0) {
-                    tmem_ld32_async(tO + c, o);
-                    tmem_loads_done();
-                    pin32(o);
-                }
-                if (mine) {
-                    uint32_t w[16];
+                        for (int c = 0; c < HD; c += 32) {
+                            float o[32];
+                            uint32_t x[32];
+                            tmem_ld32_async(tO + c, o);
+                            tmem_loads_done();
+                            pin32(o);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) w[i] = il == 0.f ? 0u : pack2<T>(o[2 * i] * il, o[2 * i + 1] * il);
-                    uint4* dst = reinterpret_cast<uint4*>(row + c);
+                            for (int i = 0; i < 32; i++) x[i] = __float_as_uint(o[i] * alpha);
+                            tmem_st32_async(tO + c, x);
+                        }
+                    }
+                    const int iv = i0 + 2 * j + 1;
+                    if ((j + 1) * BN > w.lk &&
+                        __all_sync(0xffffffffu, wait_or_abort(&full[iv % S], (iv / S) & 1, p.status, &abort_flag))) {
+                        // rows behind the sequence's last key may hold anything: zero them in V, so that
+                        // weight 0 times them is 0 (both tiles write the same zeros, each before its product)
+                        uint8_t* vb = smem + L::kKV + (iv % S) * L::kTileBytes;
+                        const int r0 = w.lk - j * BN, cnt = (BN - r0) * L::NC * 8;
+                        for (int i = r; i < cnt; i += BM) {
+                            const int row = r0 + i / (L::NC * 8), rem = i % (L::NC * 8);
+                            *reinterpret_cast<uint4*>(vb + (rem >> 3) * BN * 128 + row * 128 + (rem & 7) * 16) =
+                                make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                    }
+                    const float neg = m == -INFINITY ? 0.f : -m;  // a lane that sees nothing yet: weights 0
+                    const float2 sc = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                    for (int i = 0; i < 4; i++) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t x[32];
+#pragma unroll
+                        for (int k = 0; k < 32; k++) {
+                            const float2 y = fma2(make_float2(s[64 * h + 2 * k], s[64 * h + 2 * k + 1]), sc, off);
+                            const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                            sum[k & 1] = add2(sum[k & 1], e);
+                            x[k] = pack2<T>(e.x, e.y);
+                        }
+                        tmem_st32_async(tS + 32 * h, x);
+                        tmem_stores_done();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_full[t][h]);
+                    }
+                    sum[0] = add2(sum[0], sum[1]);
+                    l += sum[0].x + sum[0].y;
                 }
+                if (!ok) break;
+                if (nt > 0) {
+                    ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[t], no & 1, p.status, &abort_flag));
+                    if (!ok) break;
+                    no++;
+                    tc_fence_after();
+                }
+                if (toks > 0) {
+                    const float il = l > 0.f || l != l ? 1.f / l : 0.f;
+                    const bool mine = r < toks * G;
+                    T* row = static_cast<T*>(p.out) + ((int64_t)(w.q0 + tok) * p.n_heads + w.kvh * G + r % G) * HD;
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32) {
+                        float o[32];
+                        if (nt > 0) {
+                            tmem_ld32_async(tO + c, o);
+                            tmem_loads_done();
+                            pin32(o);
+                        }
+                        if (mine) {
+                            uint32_t x[16];
+#pragma unroll
+                            for (int i = 0; i < 16; i++) x[i] = il == 0.f ? 0u : pack2<T>(o[2 * i] * il, o[2 * i + 1] * il);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 8) store32(row + c + 2 * i, x + i);
+                        }
+                    }
+                }
+                i0 += 2 * w.ntot;
             }
+            index = next_item(n);
         }
     }
     tc_fence_before();
@@ -391,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <typename T, int HD>
-cudaError_t launch(const AttnPacked& a, const Params& p, cudaStream_t st) {
+cudaError_t launch(const AttnPacked& a, Params p, cudaStream_t st) {
     const int G = a.n_heads / a.n_kv;
     CUtensorMap tq, tk, tv;
     const bool bf = std::is_same<T, __nv_bfloat16>::value;
@@ -402,6 +511,7 @@ cudaError_t launch(const AttnPacked& a, const Params& p, cudaStream_t st) {
     if (a.n_k == 0) tk = tv = tq;  // no key: no copy is made
     const int64_t pairs = ceil_div64(std::min(a.max_q, a.n_q), 2 * p.tokens), ctas = pairs * a.n_kv * a.n_seq;
     if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    p.pairs = (int)pairs;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kThreads);

@@ -745,8 +745,8 @@ TPTC_API int tptc_attn_packed(int type, const void* d_q, int64_t q_stride, const
     if (n_seq < 0 || n_q < 0 || n_k < 0 || max_q < 0 || n_q > INT32_MAX - 512 || n_k > INT32_MAX - 512)
         return fail_code(nullptr, TPTC_ERR_ARG, "attn_packed: bad row counts");
     if (bad_rows(d_q, q_stride, (int64_t)n_heads * head_dim, type) || bad_rows(d_k, k_stride, (int64_t)n_kv * head_dim, type) ||
-        bad_rows(d_v, v_stride, (int64_t)n_kv * head_dim, type) || misaligned(d_out, 16))
-        return fail_code(nullptr, TPTC_ERR_ARG, "attn_packed: rows must be 16-byte aligned and not overlap");
+        bad_rows(d_v, v_stride, (int64_t)n_kv * head_dim, type) || misaligned(d_out, 32))
+        return fail_code(nullptr, TPTC_ERR_ARG, "attn_packed: rows must be 16-byte aligned (out: 32) and not overlap");
     if (n_seq == 0 || n_q == 0 || max_q == 0) return TPTC_OK;
     int dev = 0, sms = 0;
     if (int rc = ensure_kernels(&dev, &sms)) return rc;
