@@ -5,12 +5,19 @@
 //
 // Tile: 128 TMEM lanes hold floor(128 / G) consecutive tokens x the G heads of one kv head, so every
 // lane is in use for short prompts too and a K/V tile is shared by the whole group.  A CTA owns two
-// such tiles, A and B, and streams 128-key tiles of K and V through one ring: while the
-// softmax warps of one tile work, the tensor core works for the other.
-// TMEM: S_A, S_B (128 columns each), O_A, O_B.  The weights P overwrite the scores' columns as
-// 16-bit pairs and enter the second product as its TMEM operand, so they never pass through shared
-// memory.  Per pair of tiles and 128 keys (hd 128): 2048 tensor cycles and, at 16 exponentials per
-// cycle and SM, 2048 exponential cycles: both bound it.
+// such tiles, A and B, which stream the same tiles of K and V through one ring, each with its own
+// issuing warp and its own softmax warpgroup.
+// TMEM holds for both tiles the scores S (BN columns), the weights P as 16-bit pairs (BN / 2) and O (HD):
+// with P beside S and not in its place, the scores of the next keys are computed while the
+// exponentials of these run.  BN is what then fits 512 columns (128, 96, 80 keys for head_dim 64, 96,
+// 128).  P enters its product from TMEM.
+// Bounds, per pair of tiles and 128 keys at head_dim 128: 2048 cycles of exponentials (16 per cycle and
+// SM) and 2350 of the tensor core (S waits for shared memory, 6.5 KB of operands per 40 cycles).  What is
+// reached is 3450: a lone softmax warp's chain of waits, loads, maximum, exponentials and stores.
+// Tried and slower: two threads per lane (519 us for 8192 tokens, 32 heads on 8, against 441), a quarter of the exponentials
+// as polynomials (483 against 462), P in the place of S with 128 keys per tile (448), turns of A
+// and B at the exponentials (470).
+// Measured there: 441 us = 1245 TFLOP/s.
 //
 // Softmax: one thread per lane, base 2, with a reference maximum that moves (rescaling O in TMEM and
 // the f32 sum) only when a tile's maximum passes it by 8, so P stays below 2^8.
@@ -26,8 +33,8 @@ namespace tptc {
 
 namespace {
 
-constexpr int BM = 128, BN = 128;
-constexpr int kThreads = 384;  // warpgroup 0: copies (warp 0) and products (warp 1); 1 and 2: the softmax of A and B
+constexpr int BM = 128;
+constexpr int kThreads = 384;  // warpgroup 0: copies (warp 0), products of A and B (1, 2); 1 and 2: their softmax
 // Registers: 384 threads launch with 168 each; the softmax threads hold 128 scores and take what
 // warpgroup 0 gives back (128 x (72 + 2 x 216) = 384 x 168).
 constexpr int kRegsFew = 72, kRegsMany = 216;
@@ -35,11 +42,16 @@ constexpr int kTmemCols = 512;
 
 template <int HD>
 struct Lay {
+    static constexpr int BN = HD == 64 ? 128 : HD == 96 ? 96 : 80;  // keys per tile
+    static constexpr int kFirst = HD == 128 ? 80 : 64;  // weights handed over at once, then the rest (measured)
+    static constexpr int kP = 2 * BN, kO = 3 * BN;     // TMEM columns: S_A, S_B from 0, P_A, P_B, O_A, O_B
     static constexpr int NC = (HD + 63) / 64;          // 64-column blocks of a row (the last may be part empty)
-    static constexpr int kTileBytes = 128 * NC * 128;  // 128 rows of Q, K or V
-    static constexpr int kStages = HD == 64 ? 6 : 5;   // K and V tiles in turn
-    static constexpr int kKV = 2 * kTileBytes;
-    static constexpr int kBytes = kKV + kStages * kTileBytes;
+    static constexpr int kQTile = BM * NC * 128;       // bytes of a tile of Q
+    static constexpr int kTile = BN * NC * 128;        // of K or V
+    static constexpr int kStages = (220 * 1024 - 2 * kQTile) / kTile < 8 ? (220 * 1024 - 2 * kQTile) / kTile : 8;
+    static constexpr int kKV = 2 * kQTile;
+    static constexpr int kBytes = kKV + kStages * kTile;
+    static_assert(kO + 2 * HD <= kTmemCols && kTile % 1024 == 0 && kStages >= 5, "layout");
 };
 
 struct Params {
@@ -68,6 +80,25 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, u
         : "memory");
 }
 
+// Waits for a phase of a barrier; false, with the status set, when it does not come (a bounded number
+// of polls).  One instruction and a branch where the phase is complete: the loops of this kernel wait
+// up to ten times per tile, and with a called-out abort flag and a vote in each wait 8192 tokens took
+// 523 us instead of 463.  A poll may sleep for 10 us, so that waiting warps leave the issue slots to the others.
+constexpr uint32_t kPolls = 1u << 22;
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int32_t* status) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .u32 n;\n mov.u32 n, %3;\n"
+        "POLL:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n @p bra DONE;\n"
+        " sub.u32 n, n, 1;\n setp.eq.u32 p, n, 0;\n @!p bra POLL;\n setp.ne.u32 p, n, 0;\n"
+        "DONE:\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "n"(kPolls), "r"(10000)
+        : "memory");
+    if (!ok && status) atomicExch(status, TPTC_ERR_TIMEOUT);
+    return ok != 0;
+}
+
 // One lane of a converged warp.  (The compiler keeps what a warp computes alike in uniform registers, where
 // the products' operands have to be; under `lane == 0` each product cost about 100 cycles to issue.)
 __device__ __forceinline__ bool elect_one() {
@@ -76,34 +107,47 @@ __device__ __forceinline__ bool elect_one() {
     return one != 0;
 }
 
-// 32 columns, not waited for; tmem_loaded() below ends the wait for all loads before it.
-__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
-          "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
-          "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
-        : "r"(taddr));
+// N columns, not waited for; tmem_loads_done() ends the wait for all loads before it.
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float* r) {
+    static_assert(N == 16 || N == 32, "columns");
+    if constexpr (N == 16)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                     : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+                     : "r"(taddr));
+    if constexpr (N == 32)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                     : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+                     : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_loads_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // Keeps the uses of loaded registers behind the wait.
-__device__ __forceinline__ void pin32(float* r) {
+__device__ __forceinline__ void pin16(float* r) {
     asm volatile("" : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
                  "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]));
-    asm volatile("" : "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
-                 "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31]));
 }
-__device__ __forceinline__ void tmem_st32_async(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t* r) {
+    static_assert(N == 8 || N == 16 || N == 32, "columns");
+    if constexpr (N == 8)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+    if constexpr (N == 16)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+    if constexpr (N == 32)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+// N columns, a multiple of 8.
+template <int N>
+__device__ __forceinline__ void store_p(uint32_t taddr, const uint32_t* r) {
+    if constexpr (N >= 32) {
+        tmem_st<32>(taddr, r);
+        if constexpr (N > 32) store_p<N - 32>(taddr + 32, r + 32);
+    } else if constexpr (N >= 16) {
+        tmem_st<16>(taddr, r);
+        if constexpr (N > 16) store_p<N - 16>(taddr + 16, r + 16);
+    } else {
+        tmem_st<8>(taddr, r);
+    }
 }
 __device__ __forceinline__ void tmem_stores_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -117,6 +161,11 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* r) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                  "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 // Two f32 fused multiply-adds or sums in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -166,6 +215,7 @@ struct Item {
     int toks[2], nt[2], ntot;  // tokens of a tile, and the key tiles that its last token sees
 };
 // Every role decodes an item for itself, alike; false: nothing to do.
+template <int BN>
 __device__ __forceinline__ bool decode(const Params& p, int index, Item& w) {
     // the pairs of tiles with the most keys first
     const int per = p.n_kv * p.n_seq, pair = p.pairs - 1 - index / per, at = index % per, b = at / p.n_kv;
@@ -197,43 +247,44 @@ __global__ void __launch_bounds__(kThreads, 1)
     attn_packed_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                        const __grid_constant__ CUtensorMap tv, const __grid_constant__ Params p) {
     using L = Lay<HD>;
-    constexpr int S = L::kStages, KS = HD / 16;
+    constexpr int S = L::kStages, KS = HD / 16, BN = L::BN;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t q_full, q_empty, full[S], empty[S], s_full[2], p_full[2][2], o_done[2], drain, item_full[2], item_empty[2];
+    __shared__ uint64_t q_full, q_empty, full[S], empty[S], item_full[2], item_empty[2];
+    __shared__ uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2], drain[2];
     __shared__ uint4 response[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ volatile int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = p.n_heads / p.n_kv;
 
     if (threadIdx.x == 0) {
         mbar_init(&q_full, 1);
-        mbar_init(&q_empty, 1);
+        mbar_init(&q_empty, 2);  // both tiles' products are through with it
         for (int s = 0; s < S; s++) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+            mbar_init(&empty[s], 2);
         }
         for (int t = 0; t < 2; t++) {
             mbar_init(&s_full[t], 1);
-            for (int h = 0; h < 2; h++) mbar_init(&p_full[t][h], 4);  // one arrival per softmax warp
-            mbar_init(&o_done[t], 1);
+            mbar_init(&s_free[t], 4);  // one arrival per softmax warp
+            for (int h = 0; h < 2; h++) mbar_init(&p_full[t][h], 4);
+            mbar_init(&pv_done[t], 1);
+            mbar_init(&drain[t], 1);
             mbar_init(&item_full[t], 1);
-            mbar_init(&item_empty[t], 9);  // the product warp and eight softmax warps have read it
+            mbar_init(&item_empty[t], 10);  // two product warps and eight softmax warps have read it
         }
-        mbar_init(&drain, 1);
         fence_mbar_init();
-        abort_flag = 0;
     }
     if (warp == 1) tmem_alloc(&tmem_slot, kTmemCols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_phase(bar, parity, p.status); };
     // the next item's index for a warp of the products or the softmax, which has had n of them (-1: no more)
     auto next_item = [&](int n) {
         const int s = (n - 1) & 1;
-        if (!__all_sync(0xffffffffu, wait_or_abort(&item_full[s], ((n - 1) >> 1) & 1, p.status, &abort_flag))) return -1;
+        if (!wait(&item_full[s], ((n - 1) >> 1) & 1)) return -1;
         const int index = taken_item(&response[s]);
         fence_proxy_async_smem();  // read before the slot is written again
         __syncwarp();
@@ -249,8 +300,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             int index = blockIdx.x;
             for (int n = 1; ok; n++) {
                 Item w;
-                if (decode(p, index, w) && w.ntot > 0) {
-                    if (nq > 0) ok = wait_or_abort(&q_empty, (nq - 1) & 1, p.status, &abort_flag);
+                if (decode<BN>(p, index, w) && w.ntot > 0) {
+                    if (nq > 0) ok = mbar_wait_backoff(&q_empty, (nq - 1) & 1, p.status);
                     if (!ok) break;
                     nq++;
                     mbar_expect_tx(&q_full, (w.toks[1] > 0 ? 2 : 1) * ((uint32_t)(p.tokens * G) * 128 * L::NC));
@@ -258,237 +309,263 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (w.toks[t] == 0) continue;
 #pragma unroll
                         for (int c = 0; c < L::NC; c++)
-                            tma_load_3d(smem + t * L::kTileBytes + c * BM * 128, &tq, c * 64, w.kvh * G, w.q0 + t * p.tokens,
-                                        &q_full);
+                            tma_load_3d(smem + t * L::kQTile + c * BM * 128, &tq, c * 64, w.kvh * G, w.q0 + t * p.tokens, &q_full);
                     }
                     for (int k = 0; k < 2 * w.ntot; k++, i0++) {
                         const int s = i0 % S;
-                        if (i0 >= S) ok = wait_or_abort(&empty[s], ((i0 / S) - 1) & 1, p.status, &abort_flag);
+                        if (i0 >= S) ok = mbar_wait_backoff(&empty[s], ((i0 / S) - 1) & 1, p.status);
                         if (!ok) break;
-                        mbar_expect_tx(&full[s], L::kTileBytes);
+                        mbar_expect_tx(&full[s], L::kTile);
 #pragma unroll
                         for (int c = 0; c < L::NC; c++)
-                            tma_load_3d(smem + L::kKV + s * L::kTileBytes + c * BN * 128, (k & 1) ? &tv : &tk, c * 64, w.kvh,
+                            tma_load_3d(smem + L::kKV + s * L::kTile + c * BN * 128, (k & 1) ? &tv : &tk, c * 64, w.kvh,
                                         w.k0 + (k >> 1) * BN, &full[s]);
                     }
                     if (!ok) break;
                 }
                 const int s = (n - 1) & 1;
-                if (n > 2) ok = wait_or_abort(&item_empty[s], ((n - 3) >> 1) & 1, p.status, &abort_flag);
+                if (n > 2) ok = mbar_wait_backoff(&item_empty[s], ((n - 3) >> 1) & 1, p.status);
                 if (!ok) break;
                 request_item(&response[s], &item_full[s]);
-                ok = wait_or_abort(&item_full[s], ((n - 1) >> 1) & 1, p.status, &abort_flag);
+                ok = mbar_wait_backoff(&item_full[s], ((n - 1) >> 1) & 1, p.status);
                 if (!ok) break;
                 index = taken_item(&response[s]);
                 if (index < 0) break;
             }
             // the copies still in flight land before the CTA exits
-            if (nq > 0) mbar_wait_bounded(&q_full, (nq - 1) & 1, nullptr);
-            for (int k = i0 > S ? i0 - S : 0; k < i0; k++) mbar_wait_bounded(&full[k % S], (k / S) & 1, nullptr);
+            if (nq > 0) wait_phase(&q_full, (nq - 1) & 1, nullptr);
+            for (int k = i0 > S ? i0 - S : 0; k < i0; k++) wait_phase(&full[k % S], (k / S) & 1, nullptr);
         }
-        if (warp == 1) {  // products: the whole warp waits, one elected lane issues
+        if (warp == 1 || warp == 2) {  // products of a tile: the whole warp waits, one elected lane issues
+            const int t = warp - 1;
             constexpr uint32_t type_bits = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
             constexpr uint32_t id_s = mma_idesc(BM, BN) | type_bits, id_o = mma_idesc(BM, HD) | kIdescBMajorMN | type_bits;
             // (descriptors hold the address / 16 in their low bits: steps inside a tile are added there)
-            const uint64_t q_desc = sw128_desc(smem_u32(smem)), k_desc = sw128_desc(smem_u32(smem + L::kKV));
+            const uint64_t q_desc = sw128_desc(smem_u32(smem + t * L::kQTile)), k_desc = sw128_desc(smem_u32(smem + L::kKV));
             const uint64_t v_desc = sw128_desc_mn(smem_u32(smem + L::kKV), BN * 128);
+            const uint32_t tS = tmem + t * BN, tP = tmem + L::kP + t * (BN / 2), tO = tmem + L::kO + t * HD;
             const bool one = elect_one();
-            auto wait = [&](uint64_t* bar, uint32_t parity) {
-                return __all_sync(0xffffffffu, wait_or_abort(bar, parity, p.status, &abort_flag)) != 0;
-            };
+            int i0 = 0, nq = 0, ns = 0, np = 0;  // loads, Q tiles, scores and weights so far
             auto wait_full = [&](int i) { return wait(&full[i % S], (i / S) & 1); };
-            auto issue_s = [&](int t, int i) {  // i: the load of K
-                const uint64_t qa = q_desc + t * (L::kTileBytes / 16), ka = k_desc + i % S * (L::kTileBytes / 16);
-                if (one) {
-#pragma unroll
-                    for (int k = 0; k < KS; k++) {
-                        const int at = ((k / 4) * BN * 128 + 32 * (k % 4)) / 16;
-                        mma_f16(tmem + BN * t, qa + at, ka + at, id_s, k != 0);
-                    }
-                    mma_commit(&s_full[t]);
-                }
-            };
-            auto issue_pv = [&](int t, int i, bool first, int half) {  // i: the load of V
-                const uint64_t va = v_desc + i % S * (L::kTileBytes / 16);
-                if (one) {
-#pragma unroll
-                    for (int k = half * (BN / 32); k < (half + 1) * (BN / 32); k++)
-                        mma_ts(tmem + 256 + 128 * t, tmem + BN * t + 8 * k, va + k * (2048 / 16), id_o, !first || k != 0);
-                }
-            };
             auto commit = [&](uint64_t* bar) {
                 if (one) mma_commit(bar);
             };
-            int i0 = 0, nq = 0, np[2] = {0, 0};  // loads, Q tiles and weight tiles before this item
+            auto issue_s = [&](int i) {  // i: the load of K; the last scores have been taken up
+                if (ns > 0 && !wait(&s_free[t], (ns - 1) & 1)) return false;
+                ns++;
+                tc_fence_after();
+                const uint64_t ka = k_desc + i % S * (L::kTile / 16);
+                if (one) {
+#pragma unroll
+                    for (int k = 0; k < KS; k++)
+                        mma_f16(tS, q_desc + ((k / 4) * BM * 128 + 32 * (k % 4)) / 16,
+                                ka + ((k / 4) * BN * 128 + 32 * (k % 4)) / 16, id_s, k != 0);
+                    mma_commit(&s_full[t]);
+                }
+                return true;
+            };
+            auto issue_pv = [&](int i, bool first) {  // i: the load of V; the weights come in two parts
+                const uint64_t va = v_desc + i % S * (L::kTile / 16);
+#pragma unroll
+                for (int h = 0; h < (L::kFirst < BN ? 2 : 1); h++) {
+                    if (!wait(&p_full[t][h], np & 1)) return false;
+                    tc_fence_after();
+                    if (one) {
+#pragma unroll
+                        for (int k = h ? L::kFirst / 16 : 0; k < (h ? BN : L::kFirst) / 16; k++)
+                            mma_ts(tO, tP + 8 * k, va + k * (2048 / 16), id_o, !first || k != 0);
+                    }
+                }
+                np++;
+                commit(&pv_done[t]);
+                return true;
+            };
             bool ok = true;
             int index = blockIdx.x;
-            for (int n = 1; index >= 0; n++) {
-                Item w;
-                if (decode(p, index, w) && w.ntot > 0) {
-                    ok = wait(&q_full, nq & 1) && wait_full(i0);
-                    if (!ok) break;
-                    nq++;
-                    tc_fence_after();
-                    for (int t = 0; t < 2; t++)
-                        if (w.nt[t] > 0) issue_s(t, i0);
-                    commit(&empty[i0 % S]);
-                    if (w.ntot == 1) commit(&q_empty);
-                    for (int j = 0; j < w.ntot && ok; j++) {
-                        const bool more = j + 1 < w.ntot;
-                        const int iv = i0 + 2 * j + 1, ik = iv + 1;
-                        ok = wait_full(iv) && (!more || wait_full(ik));
-                        for (int t = 0; t < 2 && ok; t++) {
-                            if (j >= w.nt[t]) continue;
-                            // the weights come in two halves
-                            ok = wait(&p_full[t][0], np[t] & 1);
-                            if (!ok) break;
-                            tc_fence_after();
-                            issue_pv(t, iv, j == 0, 0);
-                            ok = wait(&p_full[t][1], np[t] & 1);
-                            if (!ok) break;
-                            tc_fence_after();
-                            issue_pv(t, iv, j == 0, 1);
-                            np[t]++;
-                            if (j + 1 < w.nt[t]) issue_s(t, ik);
-                            else commit(&o_done[t]);
-                        }
-                        if (ok) {  // V_j and K_(j + 1) are used up; Q with the last of them
-                            commit(&empty[iv % S]);
-                            if (more) commit(&empty[ik % S]);
-                            if (j + 2 == w.ntot) commit(&q_empty);
-                        }
-                    }
-                    if (!ok) break;
-                    i0 += 2 * w.ntot;
+            Item w, next;
+            bool work = decode<BN>(p, index, w), next_work = false;
+            for (int n = 1; index >= 0; n++, work = next_work, w = next) {
+                if (!work || w.ntot == 0) {
+                    index = next_item(n);
+                    next_work = index >= 0 && decode<BN>(p, index, next);
+                    continue;
                 }
-                index = next_item(n);
+                const int nt = t ? w.nt[1] : w.nt[0];
+                ok = wait(&q_full, nq & 1) && wait_full(i0);
+                if (!ok) break;
+                nq++;
+                if (nt > 0) ok = issue_s(i0);
+                commit(&empty[i0 % S]);
+                if (w.ntot == 1) commit(&q_empty);
+                for (int j = 0; j < w.ntot && ok; j++) {
+                    const int iv = i0 + 2 * j + 1, ik = iv + 1;
+                    if (j + 1 < w.ntot) {
+                        ok = wait_full(ik);
+                        if (ok && j + 1 < nt) ok = issue_s(ik);
+                        if (!ok) break;
+                        commit(&empty[ik % S]);
+                        if (j + 2 == w.ntot) commit(&q_empty);
+                    } else {  // the loads are all issued: the next item is known soon
+                        index = next_item(n);
+                        next_work = index >= 0 && decode<BN>(p, index, next);
+                    }
+                    ok = wait_full(iv);
+                    if (ok && j < nt) ok = issue_pv(iv, j == 0);
+                    if (ok) commit(&empty[iv % S]);
+                }
+                if (!ok) break;
+                i0 += 2 * w.ntot;
             }
             // every product issued has completed before TMEM is freed
-            commit(&drain);
-            mbar_wait_bounded(&drain, 0, nullptr);
+            commit(&drain[t]);
+            wait_phase(&drain[t], 0, nullptr);
             __syncwarp();
         }
     } else {  // one thread per lane of tile A or B
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
         const int t = (warp >> 2) - 1, r = 32 * (warp & 3) + lane;
         const uint32_t loff = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t tS = tmem + BN * t + loff, tO = tmem + 256 + 128 * t + loff;
-        int i0 = 0, ns = 0, no = 0;  // loads, score tiles and outputs before this item
+        const uint32_t tS = tmem + t * BN + loff, tP = tmem + L::kP + t * (BN / 2) + loff, tO = tmem + L::kO + t * HD + loff;
+        int i0 = 0, ns = 0;  // loads and score tiles so far
         bool ok = true;
         int index = blockIdx.x;
-        for (int n = 1; index >= 0; n++) {
-            Item w;
-            if (decode(p, index, w)) {
-                const int nt = t ? w.nt[1] : w.nt[0], toks = t ? w.toks[1] : w.toks[0];
-                const int tok = t * p.tokens + min(r / G, max(toks - 1, 0));  // spare lanes follow the last token
-                const int sees = w.base + tok + 1, all_see = w.base + t * p.tokens + 1;  // keys of this lane, and of every lane
-                float m = -INFINITY, l = 0.f;
-                for (int j = 0; j < nt; j++, ns++) {
-                    ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[t], ns & 1, p.status, &abort_flag));
+        Item w, next;
+        bool work = decode<BN>(p, index, w), next_work = false;
+        for (int n = 1; index >= 0; n++, work = next_work, w = next) {
+            if (!work) {
+                index = next_item(n);
+                next_work = index >= 0 && decode<BN>(p, index, next);
+                continue;
+            }
+            const int nt = t ? w.nt[1] : w.nt[0], toks = t ? w.toks[1] : w.toks[0];
+            const int tok = t * p.tokens + min(r / G, max(toks - 1, 0));  // spare lanes follow the last token
+            const int sees = w.base + tok + 1, all_see = w.base + t * p.tokens + 1;  // keys of this lane, and of every lane
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < nt; j++, ns++) {
+                ok = wait(&s_full[t], ns & 1);
+                if (!ok) break;
+                tc_fence_after();
+                float s[BN];
+#pragma unroll
+                for (int c = 0; c + 32 <= BN; c += 32) tmem_ld<32>(tS + c, s + c);
+                if constexpr (BN % 32 != 0) tmem_ld<16>(tS + BN / 32 * 32, s + BN / 32 * 32);
+                tmem_loads_done();
+#pragma unroll
+                for (int c = 0; c < BN; c += 16) pin16(s + c);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_free[t]);
+                if ((j + 1) * BN > all_see) {
+                    const int left = sees - j * BN;
+#pragma unroll
+                    for (int k = 0; k < BN; k++) s[k] = k < left ? s[k] : -INFINITY;
+                }
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int k = 4; k < BN; k += 8)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) mx[c] = k + 4 + c < BN ? max3(mx[c], s[k + c], s[k + 4 + c]) : fmaxf(mx[c], s[k + c]);
+                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                const bool move = mt > m + 8.f;
+                float alpha = 1.f;
+                if (move) {
+                    alpha = ex2(m - mt);
+                    l *= alpha;
+                    m = mt;
+                }
+                const float neg = m == -INFINITY ? 0.f : -m;  // a lane that sees nothing yet: weights 0
+                const float2 sc = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                uint32_t x[BN / 2];
+                auto weights = [&](int k0, int k1) {
+#pragma unroll
+                    for (int k = k0; k < k1; k++) {
+                        const float2 y = fma2(make_float2(s[2 * k], s[2 * k + 1]), sc, off);
+                        const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                        sum[k & 1] = add2(sum[k & 1], e);
+                        x[k] = pack2<T>(e.x, e.y);
+                    }
+                };
+                auto hand_over = [&](int h) {
+                    tmem_stores_done();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[t][h]);
+                };
+                weights(0, L::kFirst / 2);
+                // the last product has taken up P and added to O
+                if (j > 0) {
+                    ok = wait(&pv_done[t], (ns - 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    float s[BN];
-#pragma unroll
-                    for (int c = 0; c < BN; c += 32) tmem_ld32_async(tS + c, s + c);
-                    tmem_loads_done();
-#pragma unroll
-                    for (int c = 0; c < BN; c += 32) pin32(s + c);
-                    if ((j + 1) * BN > all_see) {
-                        const int left = sees - j * BN;
-#pragma unroll
-                        for (int k = 0; k < BN; k++) s[k] = k < left ? s[k] : -INFINITY;
-                    }
-                    float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                    for (int k = 4; k < BN; k++) mx[k & 3] = fmaxf(mx[k & 3], s[k]);
-                    const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-                    const bool move = mt > m + 8.f;
-                    float alpha = 1.f;
-                    if (move) {
-                        alpha = ex2(m - mt);
-                        l *= alpha;
-                        m = mt;
-                    }
-                    if (j > 0 && __any_sync(0xffffffffu, move)) {
+                    if (__any_sync(0xffffffffu, move)) {
 #pragma unroll 1
                         for (int c = 0; c < HD; c += 32) {
                             float o[32];
-                            uint32_t x[32];
-                            tmem_ld32_async(tO + c, o);
+                            uint32_t z[32];
+                            tmem_ld<32>(tO + c, o);
                             tmem_loads_done();
-                            pin32(o);
+                            pin16(o);
+                            pin16(o + 16);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) x[i] = __float_as_uint(o[i] * alpha);
-                            tmem_st32_async(tO + c, x);
-                        }
-                    }
-                    const int iv = i0 + 2 * j + 1;
-                    if ((j + 1) * BN > w.lk &&
-                        __all_sync(0xffffffffu, wait_or_abort(&full[iv % S], (iv / S) & 1, p.status, &abort_flag))) {
-                        // rows behind the sequence's last key may hold anything: zero them in V, so that
-                        // weight 0 times them is 0 (both tiles write the same zeros, each before its product)
-                        uint8_t* vb = smem + L::kKV + (iv % S) * L::kTileBytes;
-                        const int r0 = w.lk - j * BN, cnt = (BN - r0) * L::NC * 8;
-                        for (int i = r; i < cnt; i += BM) {
-                            const int row = r0 + i / (L::NC * 8), rem = i % (L::NC * 8);
-                            *reinterpret_cast<uint4*>(vb + (rem >> 3) * BN * 128 + row * 128 + (rem & 7) * 16) =
-                                make_uint4(0, 0, 0, 0);
-                        }
-                        fence_proxy_async_smem();
-                    }
-                    const float neg = m == -INFINITY ? 0.f : -m;  // a lane that sees nothing yet: weights 0
-                    const float2 sc = make_float2(p.scale_log2, p.scale_log2), off = make_float2(neg, neg);
-                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t x[32];
-#pragma unroll
-                        for (int k = 0; k < 32; k++) {
-                            const float2 y = fma2(make_float2(s[64 * h + 2 * k], s[64 * h + 2 * k + 1]), sc, off);
-                            const float2 e = make_float2(ex2(y.x), ex2(y.y));
-                            sum[k & 1] = add2(sum[k & 1], e);
-                            x[k] = pack2<T>(e.x, e.y);
-                        }
-                        tmem_st32_async(tS + 32 * h, x);
-                        tmem_stores_done();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&p_full[t][h]);
-                    }
-                    sum[0] = add2(sum[0], sum[1]);
-                    l += sum[0].x + sum[0].y;
-                }
-                if (!ok) break;
-                if (nt > 0) {
-                    ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[t], no & 1, p.status, &abort_flag));
-                    if (!ok) break;
-                    no++;
-                    tc_fence_after();
-                }
-                if (toks > 0) {
-                    const float il = l > 0.f || l != l ? 1.f / l : 0.f;
-                    const bool mine = r < toks * G;
-                    T* row = static_cast<T*>(p.out) + ((int64_t)(w.q0 + tok) * p.n_heads + w.kvh * G + r % G) * HD;
-#pragma unroll
-                    for (int c = 0; c < HD; c += 32) {
-                        float o[32];
-                        if (nt > 0) {
-                            tmem_ld32_async(tO + c, o);
-                            tmem_loads_done();
-                            pin32(o);
-                        }
-                        if (mine) {
-                            uint32_t x[16];
-#pragma unroll
-                            for (int i = 0; i < 16; i++) x[i] = il == 0.f ? 0u : pack2<T>(o[2 * i] * il, o[2 * i + 1] * il);
-#pragma unroll
-                            for (int i = 0; i < 16; i += 8) store32(row + c + 2 * i, x + i);
+                            for (int i = 0; i < 32; i++) z[i] = __float_as_uint(o[i] * alpha);
+                            tmem_st<32>(tO + c, z);
                         }
                     }
                 }
-                i0 += 2 * w.ntot;
+                const int iv = i0 + 2 * j + 1;
+                if ((j + 1) * BN > w.lk && wait(&full[iv % S], (iv / S) & 1)) {
+                    // rows behind the sequence's last key may hold anything: zero them in V, so that
+                    // weight 0 times them is 0 (both tiles write the same zeros, each before its product)
+                    uint8_t* vb = smem + L::kKV + (iv % S) * L::kTile;
+                    const int r0 = w.lk - j * BN, cnt = (BN - r0) * L::NC * 8;
+                    for (int i = r; i < cnt; i += BM) {
+                        const int row = r0 + i / (L::NC * 8), rem = i % (L::NC * 8);
+                        *reinterpret_cast<uint4*>(vb + (rem >> 3) * BN * 128 + row * 128 + (rem & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                }
+                store_p<L::kFirst / 2>(tP, x);
+                hand_over(0);
+                if constexpr (L::kFirst < BN) {
+                    weights(L::kFirst / 2, BN / 2);
+                    store_p<(BN - L::kFirst) / 2>(tP + L::kFirst / 2, x + L::kFirst / 2);
+                    hand_over(1);
+                }
+                sum[0] = add2(sum[0], sum[1]);
+                l += sum[0].x + sum[0].y;
             }
+            if (!ok) break;
             index = next_item(n);
+            next_work = index >= 0 && decode<BN>(p, index, next);
+            if (nt > 0) {
+                ok = wait(&pv_done[t], (ns - 1) & 1);
+                if (!ok) break;
+                tc_fence_after();
+            }
+            if (toks > 0) {
+                const float il = l > 0.f || l != l ? 1.f / l : 0.f;
+                const bool mine = r < toks * G;
+                T* row = static_cast<T*>(p.out) + ((int64_t)(w.q0 + tok) * p.n_heads + w.kvh * G + r % G) * HD;
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) {
+                    float o[32];
+                    if (nt > 0) {
+                        tmem_ld<32>(tO + c, o);
+                        tmem_loads_done();
+                        pin16(o);
+                        pin16(o + 16);
+                    }
+                    if (mine) {
+                        uint32_t z[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) z[i] = il == 0.f ? 0u : pack2<T>(o[2 * i] * il, o[2 * i + 1] * il);
+#pragma unroll
+                        for (int i = 0; i < 16; i += 8) store32(row + c + 2 * i, z + i);
+                    }
+                }
+            }
+            i0 += 2 * w.ntot;
         }
     }
     tc_fence_before();
@@ -505,8 +582,8 @@ cudaError_t launch(const AttnPacked& a, Params p, cudaStream_t st) {
     CUtensorMap tq, tk, tv;
     const bool bf = std::is_same<T, __nv_bfloat16>::value;
     cudaError_t e = make_tmap_heads(&tq, a.q, bf, HD, a.n_heads, a.n_q, a.q_stride, G, p.tokens);
-    if (e == cudaSuccess && a.n_k > 0) e = make_tmap_heads(&tk, a.k, bf, HD, a.n_kv, a.n_k, a.k_stride, 1, BN);
-    if (e == cudaSuccess && a.n_k > 0) e = make_tmap_heads(&tv, a.v, bf, HD, a.n_kv, a.n_k, a.v_stride, 1, BN);
+    if (e == cudaSuccess && a.n_k > 0) e = make_tmap_heads(&tk, a.k, bf, HD, a.n_kv, a.n_k, a.k_stride, 1, Lay<HD>::BN);
+    if (e == cudaSuccess && a.n_k > 0) e = make_tmap_heads(&tv, a.v, bf, HD, a.n_kv, a.n_k, a.v_stride, 1, Lay<HD>::BN);
     if (e != cudaSuccess) return e;
     if (a.n_k == 0) tk = tv = tq;  // no key: no copy is made
     const int64_t pairs = ceil_div64(std::min(a.max_q, a.n_q), 2 * p.tokens), ctas = pairs * a.n_kv * a.n_seq;
