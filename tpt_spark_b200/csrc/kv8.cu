@@ -6,9 +6,9 @@
 // become rint(c s / s'), so a value moves by at most half a step s' each time the scale grows.
 // The maximum over the page couples all of its new rows, hence the split: one CTA per (sequence,
 // touched page, kv head), which keeps the page's rotated rows in registers between the maximum
-// and the rounding (each input is read once) and rotates the query rows of its head group and
-// positions, so one launch moves q, k and v.  Bound by HBM for prompts and by launch latency for
-// decode steps.
+// and the rounding (each input is read once).  A second CTA beside it rotates the query rows of
+// its head group and positions, four heads of a token per thread with one pair of cos and sin vectors, so one launch moves q, k and
+// v.  Bound by HBM for prompts and by launch latency for decode steps: APPTIME.
 #include <algorithm>
 
 #include "serve.h"
@@ -28,7 +28,7 @@ struct Span {
     int first, n;   // packed row of the first, and how many
     int off;        // their first row in the page
     int pos;        // position of the first
-    int page_id;    // -1: not in the cache
+    int64_t entry;  // of the page table
 };
 __device__ __forceinline__ bool page_span(const tptc_kv8& c, const int32_t* cu, const int32_t* start, int n_rows,
                                           int most, int rope_rows, int b, int u, Span& s) {
@@ -45,58 +45,65 @@ __device__ __forceinline__ bool page_span(const tptc_kv8& c, const int32_t* cu, 
     s.n = (int)(r1 - r0);
     s.off = (int)(r0 - p * c.page);
     s.pos = (int)r0;
-    const int id = c.table[(int64_t)b * c.max_pages + p];
-    s.page_id = id >= 0 && id < c.n_pages ? id : -1;
-    if (s.page_id < 0 && threadIdx.x == 0) flag(c.status);
+    s.entry = (int64_t)b * c.max_pages + p;
     return true;
 }
 
-// Rotates elements [8 lg, 8 lg + 8) of a row held by a group of lanes (lane lg of the group holds
-// those elements).  Each product and sum is rounded by itself, as the framework's other
-// rotations do.  Every lane of the warp takes part (the halves form exchanges vectors).
+// A page id as it is (id), and whether it is in the cache; one that is not is flagged and not followed.
+__device__ __forceinline__ bool in_cache(const tptc_kv8& c, int id) {
+    const bool in = id >= 0 && id < c.n_pages;
+    if (!in && threadIdx.x == 0) flag(c.status);
+    return in;
+}
+
+// The cos and sin that the eight elements of lane lg of a row at `pos` take (pairs: four of each).
+struct Angles {
+    float c[8], s[8];
+};
+__device__ __forceinline__ void load_angles(const tptc_rope& r, int lg, int pos, bool in, Angles& a) {
+    const int e = 8 * lg, half = r.dim / 2;
+    if (!in || e >= r.dim) return;
+    const int64_t at = (int64_t)pos * half + (r.halves ? (e >= half ? e - half : e) : e / 2);
+    const float4* c = reinterpret_cast<const float4*>(r.cos + at);
+    const float4* s = reinterpret_cast<const float4*>(r.sin + at);
+    reinterpret_cast<float4*>(a.c)[0] = __ldg(c);
+    reinterpret_cast<float4*>(a.s)[0] = __ldg(s);
+    if (r.halves) {
+        reinterpret_cast<float4*>(a.c)[1] = __ldg(c + 1);
+        reinterpret_cast<float4*>(a.s)[1] = __ldg(s + 1);
+    }
+}
+
+// The eight elements of lane lg of a row (held by a group of lanes), rotated.  Each product and sum is
+// rounded by itself, as the framework's other rotations do.  Every lane of the warp takes part (the
+// halves form exchanges vectors as they were loaded; for the first half the partner's sign turns with them).
 template <typename T>
-__device__ __forceinline__ void rotate8(float (&x)[8], int lg, int pos, bool valid, const tptc_rope& r) {
-    const int c = 8 * lg;
-    const bool in = valid && c < r.dim;
+__device__ __forceinline__ void rotate8(const Raw8<T>& w, float (&x)[8], int lg, const tptc_rope& r, const Angles& a) {
+    unpack8<T>(w, x);
+    const int e = 8 * lg;
     if (!r.halves) {
-        if (!in) return;
-        const int64_t at = (int64_t)pos * (r.dim / 2) + c / 2;
-        const float4 cs = __ldg(reinterpret_cast<const float4*>(r.cos + at));
-        const float4 sn = __ldg(reinterpret_cast<const float4*>(r.sin + at));
-        const float cc[4] = {cs.x, cs.y, cs.z, cs.w}, ss[4] = {sn.x, sn.y, sn.z, sn.w};
+        if (e >= r.dim) return;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float a = x[2 * i], b = x[2 * i + 1];
-            x[2 * i] = __fsub_rn(__fmul_rn(a, cc[i]), __fmul_rn(b, ss[i]));
-            x[2 * i + 1] = __fadd_rn(__fmul_rn(a, ss[i]), __fmul_rn(b, cc[i]));
+            const float u = x[2 * i], v = x[2 * i + 1];
+            x[2 * i] = __fsub_rn(__fmul_rn(u, a.c[i]), __fmul_rn(v, a.s[i]));
+            x[2 * i + 1] = __fadd_rn(__fmul_rn(u, a.s[i]), __fmul_rn(v, a.c[i]));
         }
         return;
     }
-    const int half = r.dim / 2, delta = half / 8;
-    const bool second = c >= half;
-    const int lane = threadIdx.x & 31, src = in ? (second ? lane - delta : lane + delta) : lane;
+    const int half = r.dim / 2, delta = half / 8, lane = threadIdx.x & 31;
+    const int src = e >= r.dim ? lane : e >= half ? lane - delta : lane + delta;
+    const uint32_t sign = e >= half ? 0u : sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+    const uint32_t* wi = reinterpret_cast<const uint32_t*>(&w);
+    Raw8<T> o;
+    uint32_t* wo = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+    for (int i = 0; i < 2 * (int)sizeof(T); i++) wo[i] = __shfl_sync(0xffffffffu, wi[i], src) ^ sign;
+    if (e >= r.dim) return;
     float y[8];
-    if constexpr (sizeof(T) == 4) {
+    unpack8<T>(o, y);
 #pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = __shfl_sync(0xffffffffu, x[i], src);
-    } else {  // the values are T exactly: exchange them in pairs
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t w = __shfl_sync(0xffffffffu, pack2<T>(x[2 * i], x[2 * i + 1]), src);
-            const T* h = reinterpret_cast<const T*>(&w);
-            y[2 * i] = to_f32(h[0]), y[2 * i + 1] = to_f32(h[1]);
-        }
-    }
-    if (!in) return;
-    const int64_t at = (int64_t)pos * half + (second ? c - half : c);
-    float cc[8], ss[8];
-    load8(r.cos + at, cc);
-    load8(r.sin + at, ss);
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float xc = __fmul_rn(x[i], cc[i]), ys = __fmul_rn(y[i], ss[i]);
-        x[i] = second ? __fadd_rn(ys, xc) : __fsub_rn(xc, ys);
-    }
+    for (int i = 0; i < 8; i++) x[i] = __fadd_rn(__fmul_rn(x[i], a.c[i]), __fmul_rn(y[i], a.s[i]));
 }
 
 // Scale of a page after values of magnitude up to `top` joined it (inf or NaN: not finite).
@@ -150,31 +157,75 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
     __shared__ float s_top[2][kThreads / 32];
     const int tid = threadIdx.x, lg = tid % GS, grp = tid / GS, c = 8 * lg;
     const bool lane_in = c < HD;
-    const int h = blockIdx.x % p.c.n_kv, unit = blockIdx.x / p.c.n_kv, u = unit % p.units, b = unit / p.units;
+    const int roles = p.q_out ? 2 : 1, role = blockIdx.x % roles, rest = blockIdx.x / roles;
+    const int h = rest % p.c.n_kv, unit = rest / p.c.n_kv, u = unit % p.units, b = unit / p.units;
     Span s;
     if (!page_span(p.c, p.cu, p.start, p.n_tokens, p.max_new, p.rope.dim ? p.rope.rows : -1, b, u, s)) return;
 
+    if (role == 1) {  // the queries of this head group at the same positions: up to B heads of a token at a time
+        constexpr int B = 4;
+        const int G = p.n_heads / p.c.n_kv, sets = (G + B - 1) / B, items = s.n * sets;
+        const T* qin = static_cast<const T*>(p.q) + (int64_t)s.first * p.q_stride + (int64_t)h * G * HD + c;
+        T* qout = static_cast<T*>(p.q_out) + ((int64_t)s.first * p.n_heads + (int64_t)h * G) * HD + c;
+        for (int w0 = 0; w0 < items; w0 += RP) {
+            const int w = w0 + grp, t = sets == 1 ? w : w / sets, g0 = sets == 1 ? 0 : (w - t * sets) * B;
+            const int n = lane_in && w < items ? min(B, G - g0) : 0;
+            const T* src = qin + (int64_t)t * p.q_stride + g0 * HD;
+            T* dst = qout + ((int64_t)t * p.n_heads + g0) * HD;
+            Raw8<T> v[B];
+            Angles a;
+#pragma unroll
+            for (int i = 0; i < B; i++)
+                if (i < n) v[i] = load_raw8(src + i * HD);
+            if (p.rope.dim) load_angles(p.rope, lg, s.pos + t, n > 0, a);
+#pragma unroll
+            for (int i = 0; i < B; i++) {
+                float x[8];
+                if (p.rope.dim) rotate8<T>(v[i], x, lg, p.rope, a);
+                else unpack8<T>(v[i], x);
+                if (i < n) store8(dst + i * HD, x);
+            }
+        }
+        return;
+    }
+    const int page_id = p.c.table[s.entry];  // (looked at after the rows are on their way)
     const T* kin = static_cast<const T*>(p.k) + (int64_t)s.first * p.k_stride + h * HD + c;
     const T* vin = static_cast<const T*>(p.v) + (int64_t)s.first * p.v_stride + h * HD + c;
     float xk[NR][8], xv[NR][8];
     float top_k = 0.f, top_v = 0.f;
     bool odd_k = false, odd_v = false;  // a value that is not finite
+    {
+        Raw8<T> wk[NR], wv[NR];
 #pragma unroll
-    for (int i = 0; i < NR; i++) {
-        const int row = grp + i * RP;
-        const bool in = lane_in && row < s.n;
+        for (int i = 0; i < NR; i++) {
+            const int row = grp + i * RP;
+            wk[i] = wv[i] = Raw8<T>{};
+            if (lane_in && row < s.n) {
+                wk[i] = load_raw8(kin + row * p.k_stride);
+                wv[i] = load_raw8(vin + row * p.v_stride);
+            }
+        }
 #pragma unroll
-        for (int e = 0; e < 8; e++) xk[i][e] = xv[i][e] = 0.f;
-        if (in) {
-            load8(kin + row * p.k_stride, xk[i]);
-            load8(vin + row * p.v_stride, xv[i]);
+        for (int i = 0; i < NR; i++) {
+            const int row = grp + i * RP;
+            Angles a;
+            if (p.rope.dim) {
+                const bool in = lane_in && row < s.n;
+                load_angles(p.rope, lg, s.pos + row, in, a);
+                rotate8<T>(wk[i], xk[i], lg, p.rope, a);
+                if (!in)  // (angles that were not loaded)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) xk[i][e] = 0.f;
+            } else {
+                unpack8<T>(wk[i], xk[i]);
+            }
+            unpack8<T>(wv[i], xv[i]);
         }
     }
 #pragma unroll
     for (int i = 0; i < NR; i++) {
         const int row = grp + i * RP;
         const bool in = lane_in && row < s.n;
-        if (p.rope.dim) rotate8<T>(xk[i], lg, s.pos + row, in, p.rope);
         if (in && p.k_out)
             store8(static_cast<T*>(p.k_out) + ((int64_t)(s.first + row) * p.c.n_kv + h) * HD + c, xk[i]);
 #pragma unroll
@@ -192,24 +243,11 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_const
     top_v = warp_max(top_v);
     if ((tid & 31) == 0) s_top[0][tid >> 5] = top_k, s_top[1][tid >> 5] = top_v;
 
-    const int64_t at = (int64_t)s.page_id * p.c.n_kv + h;
-    const bool store = s.page_id >= 0;
+    const bool store = in_cache(p.c, page_id);
+    const int64_t at = (int64_t)page_id * p.c.n_kv + h;
     float old_k = 0.f, old_v = 0.f;
     if (store && s.off > 0) old_k = p.c.k_scale[at], old_v = p.c.v_scale[at];
 
-    if (p.q_out) {  // the queries of this head group at the same positions
-        const int G = p.n_heads / p.c.n_kv, rows = s.n * G;
-        const T* qin = static_cast<const T*>(p.q) + (int64_t)s.first * p.q_stride + (int64_t)h * G * HD + c;
-        T* qout = static_cast<T*>(p.q_out) + ((int64_t)s.first * p.n_heads + (int64_t)h * G) * HD + c;
-        for (int r0 = 0; r0 < rows; r0 += RP) {
-            const int r = r0 + grp, t = r / G, g = r - t * G;
-            const bool in = lane_in && r < rows;
-            float x[8] = {};
-            if (in) load8(qin + (int64_t)t * p.q_stride + g * HD, x);
-            if (p.rope.dim) rotate8<T>(x, lg, s.pos + t, in, p.rope);
-            if (in) store8(qout + ((int64_t)t * p.n_heads + g) * HD, x);
-        }
-    }
     __syncthreads();  // the maxima are in; every thread has read the old scales
     if (!store) return;
     top_k = s_top[0][0], top_v = s_top[1][0];
@@ -257,13 +295,15 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constan
     const int groups = (p.c.n_kv + p.heads_per_cta - 1) / p.heads_per_cta;
     const int g = blockIdx.x % groups, unit = blockIdx.x / groups, u = unit % p.units, b = unit / p.units;
     Span s;
-    if (!page_span(p.c, p.cu, p.start, p.n_tokens, p.max_rows, -1, b, u, s) || s.page_id < 0) return;
+    if (!page_span(p.c, p.cu, p.start, p.n_tokens, p.max_rows, -1, b, u, s)) return;
+    const int page_id = p.c.table[s.entry];
+    if (!in_cache(p.c, page_id)) return;
     const int h0 = g * p.heads_per_cta, heads = min(p.heads_per_cta, p.c.n_kv - h0);
     const int per = s.n * CH, total = heads * per;
 #pragma unroll 2
     for (int i = threadIdx.x; i < total; i += kThreads) {
         const int hh = i / per, rem = i - hh * per, row = rem / CH, ch = rem - row * CH;
-        const int64_t at = (int64_t)s.page_id * p.c.n_kv + h0 + hh;
+        const int64_t at = (int64_t)page_id * p.c.n_kv + h0 + hh;
         const int64_t src = (at * p.c.page + s.off + row) * HD + ch * 16;
         const int64_t dst = ((int64_t)(s.first + row) * p.c.n_kv + h0 + hh) * HD + ch * 16;
         if (p.k_out) {
@@ -318,7 +358,7 @@ int touched_pages(int n, int page) { return (int)(((int64_t)n + page - 2) / page
 
 cudaError_t launch_kv8_append(int type, Kv8Append p, cudaStream_t st) {
     p.units = touched_pages(std::min(p.max_new, p.n_tokens), p.c.page);
-    const int64_t ctas = (int64_t)p.c.n_seq * p.units * p.c.n_kv;
+    const int64_t ctas = (int64_t)p.c.n_seq * p.units * p.c.n_kv * (p.q_out ? 2 : 1);
     if (type == TPTC_TYPE_F16) return append_t<__half>(p, ctas, st);
     if (type == TPTC_TYPE_BF16) return append_t<__nv_bfloat16>(p, ctas, st);
     return append_t<float>(p, ctas, st);

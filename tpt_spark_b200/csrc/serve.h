@@ -6,35 +6,45 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace tptc {
 
-// Eight consecutive elements of a row as f32, whatever the element type.
+// Eight consecutive elements of a row, as loaded and as f32, whatever the element type.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-template <>
-__device__ __forceinline__ void load8<__half>(const __half* p, float (&x)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const T* p) {
+    Raw8<T> r;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
-        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& v, float (&x)[8]) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(&v);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __uint_as_float(r[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(reinterpret_cast<const __half2&>(r[i]));
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            x[2 * i] = __uint_as_float(r[i] << 16), x[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
     }
 }
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t r[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        x[2 * i] = __uint_as_float(r[i] << 16), x[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+    unpack8<T>(load_raw8(p), x);
 }
 
 // Two f32 as a pair of T in one word (round to nearest), the first in the low half.
