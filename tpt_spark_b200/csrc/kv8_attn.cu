@@ -2,16 +2,19 @@
 //
 // For key j of block (page, kv head) with scales ks, vs and codes c, d:
 //     s_j = (q . c_j) ks / sqrt(hd),     out = sum_j softmax(s)_j vs d_j.
-// Codes are integers up to 127, exact in fp16, so both products run on the tensor cores against
-// the codes themselves and each scale multiplies a 16-key tile's scores and weights afterwards.
+// S runs on the 8-bit integer tensor cores against the codes as they lie in memory: a query is written as
+// q = step (256 a + b) (f32: step (65536 a + 256 b + c)) with signed 8-bit digits, so the sums are
+// exact and q is off by at most 2^-16 (f32: 2^-23) of its largest element.  O needs weights of
+// any size and runs in fp16, where codes are exact too; each scale multiplies a 16-key tile's scores and
+// weights.
 //
-// Bound: every K and V byte is read once for the whole head group (HBM).  What the layout is
-// built around is therefore bytes in flight: 16 keys are one m16n8k16 step with the keys as M, so
-// the 8 columns carry up to 8 query heads,
+// Bound: every K and V byte is read once for the whole head group (HBM); close behind it the instructions per tile (the
+// codes of V become fp16 by byte permutes onto 1024 + 128 + c).  The layout is built around bytes in flight and
+// few instructions: 16 keys are the M of one tensor-core step, so the 8 columns carry up to 8 query heads,
 //     S^T[key][head] = K . Q^T,          O^T[dim][head] += V^T . P^T,
 // and the k indices of S and the dims of O are permuted so that each thread needs whole 16-byte
-// runs of the codes.  A thread copies exactly the bytes it will use itself (cp.async into its own slots
-// of a ring), so the loop has no barrier at all: a warp waits for its own copies only.
+// runs of the codes.  Each warp has a ring of its own (cp.async, whole runs of a page: copies that took 32 bytes
+// of a row at a time moved 1.5 times the bytes from L2), so the loop has no barrier: a warp waits for its copies only.
 //
 // Work split: the 16-key tiles of all (sequence, kv head) pairs form one line, cut into equal
 // ranges, one per CTA, so ragged batches are balanced whatever the lengths; inside a range the
@@ -21,7 +24,7 @@
 // Weights: p = 2^(x - m) with a reference m that moves only when a score passes it by 8 (f32 sum
 // l).  The tensor core takes p vs 2^(m - M) as fp16, where M is the same kind of reference for
 // x + log2 vs: pages whose scales differ by any ratio keep fp16's relative precision against the
-// largest contribution.  For f32 queries q and the weights go in as a high and a low fp16 part.
+// largest contribution.  For f32 the weights go in as a high and a low fp16 part.
 #include <math.h>
 
 #include <algorithm>
@@ -42,8 +45,8 @@ constexpr int kMinTiles = 16;   // tiles that make a CTA worth its share of the 
 
 template <int HD>
 struct Lay {
-    static constexpr int kKVec = HD == 96 ? 8 : 16;   // bytes per copy of K
-    static constexpr int kKPer = HD / 4 / kKVec;      // copies per row and thread
+    static constexpr int kKVec = HD == 96 ? 8 : 16;   // bytes of a run of K
+    static constexpr int kKPer = HD / 4 / kKVec;      // runs per row and thread
     static constexpr int kVVec = HD == 128 ? 16 : HD == 96 ? 4 : 8;
     static constexpr int kVPer = HD / 8 / kVVec;
     static constexpr int kKBytes = kTile * HD;
@@ -54,12 +57,8 @@ struct Lay {
     static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
 };
 
-template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 template <int BYTES>
@@ -78,6 +77,12 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -142,7 +147,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __grid_constant__ Params p) {
     using L = Lay<HD>;
     constexpr bool kSplit = sizeof(T) == 4;  // high and low parts
-    constexpr int KS = HD / 16, MT = HD / 16;
+    constexpr int MT = HD / 16;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int s_scan[kWarps], s_start[3];
     __shared__ int s_last;
@@ -150,12 +155,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
     const int G = p.n_heads / p.c.n_kv, subs = (G + kHeads - 1) / kHeads, pairs = p.c.n_kv * subs;
 
     // ---- this CTA's range of the line of tiles
+    auto tiles_of = [&](int b, bool report) {
+        return b < p.c.n_seq ? (length_of(p, b, report) + kTile - 1) / kTile : 0;
+    };
+    const int tiles0 = tiles_of(tid, blockIdx.x == 0);  // of the first kThreads sequences
     int64_t total = 0;
     for (int b0 = 0; b0 < p.c.n_seq; b0 += kThreads) {
-        const int b = b0 + tid;
-        int t = b < p.c.n_seq ? (length_of(p, b, blockIdx.x == 0) + kTile - 1) / kTile : 0;
-        t = warp_sum_i(t);
-        __syncthreads();
+        const int t = warp_sum_i(b0 == 0 ? tiles0 : tiles_of(b0 + tid, blockIdx.x == 0));
+        if (b0 > 0) __syncthreads();
         if (lane == 0) s_scan[warp] = t;
         __syncthreads();
         for (int w = 0; w < kWarps; w++) total += s_scan[w];
@@ -174,17 +181,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
         int64_t before = 0;  // tiles before the block of sequences
         bool found = false;
         for (int b0 = 0; b0 < p.c.n_seq && !found; b0 += kThreads) {
-            const int b = b0 + tid;
-            const int t = b < p.c.n_seq ? (length_of(p, b, false) + kTile - 1) / kTile : 0;
+            const int b = b0 + tid, t = b0 == 0 ? tiles0 : tiles_of(b, false);
             int incl = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int v = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += v;
             }
-            __syncthreads();
-            if (lane == 31) s_scan[warp] = incl;
-            __syncthreads();
+            if (p.c.n_seq > kThreads) {  // (the warps' sums are still there when one block holds all sequences)
+                __syncthreads();
+                if (lane == 31) s_scan[warp] = incl;
+                __syncthreads();
+            }
             int64_t lead = before;
             for (int w = 0; w < warp; w++) lead += s_scan[w];
             const int64_t lo = (lead + incl - t) * pairs, hi = (lead + incl) * pairs;
@@ -202,44 +210,70 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
     int len = length_of(p, b, false), tiles = (len + kTile - 1) / kTile;
 
     const uint32_t ring = smem_u32(smem) + warp * (kStages * L::kStage);
+    // Where a lane's copies go in a stage (512 bytes per copy of the warp, rows in order), and where a thread
+    // finds its runs: 16-byte chunks change places inside 128 bytes so that both are free of bank conflicts.
+    // K: rows g and g + 8; V: rows 2 t4 and 2 t4 + 1, and those behind them by 8.
+    uint32_t k_to = lane * 16, v_to = lane * 16, k_of, v_of;
+    if constexpr (HD == 128) {
+        k_to = ((lane & ~7) | ((lane & 7) ^ ((lane & 8) >> 1))) * 16;
+        v_to = ((lane & ~7) | ((lane & 7) ^ ((lane & 16) >> 3))) * 16;
+        k_of = g * 128 + (t4 ^ ((g & 1) << 2)) * 16;
+        v_of = t4 * 256 + (g ^ (t4 << 1)) * 16;
+    } else if constexpr (HD == 64) {
+        v_to = ((lane & ~7) | ((lane & 7) ^ ((lane & 24) >> 2))) * 16;
+        k_of = g * 64 + t4 * 16;
+        v_of = t4 * 128 + ((g >> 1) ^ (t4 << 1)) * 16 + (g & 1) * 8;
+    } else {
+        k_of = g * 96 + t4 * 8;
+        v_of = t4 * 192 + g * 12;
+    }
+    auto k_run = [&](int r, int j) { return r * 8 * HD + (HD == 128 ? k_of ^ (j * 64) : k_of + j * 32); };
+    auto v_run = [&](int r, int j) {
+        return (r >> 1) * 8 * HD + (HD == 64 ? v_of ^ ((r & 1) * 64) : v_of + (r & 1) * HD + j * L::kVVec);
+    };
     for (; at < end;) {
         const int n = (int)min((int64_t)(tiles - tile), end - at);  // tiles of this piece
         const int kvh = pair / subs, h0 = kvh * G + (pair % subs) * kHeads, nh = min(kHeads, kvh * G + G - h0);
 
-        // ---- the queries, as the B operand: thread holds head g, dims of its own bytes of K
-        uint32_t qh[KS][2], ql[kSplit ? KS : 1][2];
+        // ---- the queries, as the B operand: thread holds the digits of head g, dims of its own bytes of K
+        constexpr int DIGITS = kSplit ? 3 : 2, WORDS = HD / 16;  // words of four dims
+        uint32_t qd[DIGITS][WORDS];
         float fq0, fq1;
         {
             const T* q = static_cast<const T*>(p.q) + (int64_t)b * p.q_stride + (int64_t)(h0 + g) * HD;
-            float x[KS][4], top = 0.f;
+            float x[WORDS][4], top = 0.f;
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                constexpr int per = L::kKVec / 4;  // k steps per copy
+            for (int s = 0; s < WORDS; s++) {
+                constexpr int per = L::kKVec / 4;  // words per copy
                 const int d = (s / per) * (4 * L::kKVec) + t4 * L::kKVec + (s % per) * 4;
                 x[s][0] = x[s][1] = x[s][2] = x[s][3] = 0.f;
                 if (g < nh) load4(q + d, x[s]);
 #pragma unroll
-                for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[s][e]));
+                for (int e = 0; e < 4; e++) top = fmaxf(top, x[s][e] == x[s][e] ? fabsf(x[s][e]) : INFINITY);
             }
-            // a power of two that brings the largest element to [1, 2): fp16 then holds bf16 exactly
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            int e2 = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0 : (int)(__float_as_uint(top) >> 23) - 127;
-            if (!(top <= 3.402823466e38f) || top < 1.17549435e-38f) e2 = 0;
-            const float down = ldexpf(1.f, -e2);
+            // the largest element becomes 127 in its highest digit (a power of two first, so that no factor
+            // leaves f32's range); an element that is not finite makes the head's scores NaN
+            const int e2 = top < 1.17549435e-38f ? -126 : (int)(__float_as_uint(top) >> 23) - 126;
+            constexpr float kMost = kSplit ? 127.f * 65536.f : 127.f * 256.f;
+            const float down = ldexpf(1.f, -e2), unit = top * down, up = unit > 0.f ? kMost / unit : 0.f;
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
+            for (int s = 0; s < WORDS; s++) {
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const float a = x[s][2 * i] * down, c = x[s][2 * i + 1] * down;
-                    qh[s][i] = pack2<__half>(a, c);
-                    if constexpr (kSplit) {
-                        const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&qh[s][i]));
-                        ql[s][i] = pack2<__half>(a - hi.x, c - hi.y);
+                for (int d = 0; d < DIGITS; d++) qd[d][s] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    int v = __float2int_rn(x[s][e] * down * up);
+#pragma unroll
+                    for (int d = DIGITS - 1; d >= 0; d--) {  // signed digits: the carry goes on
+                        const int low = d ? (int)(int8_t)v : v;
+                        v = (v - low) >> 8;
+                        qd[d][s] |= (uint32_t)(low & 255) << (8 * e);
                     }
                 }
             }
-            const float f = ldexpf(p.scale_log2, e2);
+            const float f = top <= 3.402823466e38f ? ldexpf(p.scale_log2 * (unit / kMost), e2) : __int_as_float(0x7fc00000);
             fq0 = __shfl_sync(0xffffffffu, f, 8 * t4);
             fq1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
         }
@@ -271,26 +305,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
         fetch(1, id1, ks1, vs1);
         int batch = 0;  // id0 .. are of this batch, id1 .. of the next
 
-        auto issue = [&](int i) {
+        const int page_mask = p.c.page - 1;
+        const int64_t page_bytes = (int64_t)p.c.n_kv * p.c.page * HD;  // of all heads
+        const int8_t* k_at = p.c.k + (int64_t)kvh * p.c.page * HD + lane * 16;
+        const int8_t* v_at = p.c.v + (int64_t)kvh * p.c.page * HD + lane * 16;
+        auto issue = [&](int i, int slot) {  // 2 x 16 rows, each a run of the page
             if (i < mine) {
                 const int id = __shfl_sync(0xffffffffu, (i >> 5) == batch ? id0 : id1, i & 31);
-                const int64_t pos = (int64_t)(tile + warp + i * kWarps) * kTile;
-                const int64_t row = ((int64_t)id * p.c.n_kv + kvh) * p.c.page + pos % p.c.page;
-                const int8_t* k = p.c.k + row * HD;
-                const int8_t* v = p.c.v + row * HD;
-                const uint32_t st = ring + (i % kStages) * L::kStage;
+                const int64_t off = id * page_bytes + (((tile + warp + i * kWarps) * kTile) & page_mask) * HD;
+                const int8_t *k = k_at + off, *v = v_at + off;
+                const uint32_t kd = ring + slot * L::kStage, vd = kd + L::kKBytes;
 #pragma unroll
-                for (int r = 0; r < 2; r++)
-#pragma unroll
-                    for (int j = 0; j < L::kKPer; j++)
-                        copy_async<L::kKVec>(st + ((r * L::kKPer + j) * 32 + lane) * L::kKVec,
-                                             k + (g + 8 * r) * HD + (j * 4 + t4) * L::kKVec);
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int j = 0; j < L::kVPer; j++)
-                        copy_async<L::kVVec>(st + L::kKBytes + ((r * L::kVPer + j) * 32 + lane) * L::kVVec,
-                                             v + (2 * t4 + (r & 1) + 8 * (r >> 1)) * HD + g * (HD / 8) + j * L::kVVec);
+                for (int n = 0; n < HD / 32; n++) {
+                    copy_async(kd + n * 512 + k_to, k + n * 512);
+                    copy_async(vd + n * 512 + (HD == 128 && (n & 1) ? v_to ^ 64 : v_to), v + n * 512);
+                }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -298,11 +327,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
         float o[MT][4];
 #pragma unroll
         for (int j = 0; j < MT; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // heads 2 t4 and 2 t4 + 1
-        float r0 = -INFINITY, r1 = -INFINITY, w0 = 0.f, w1 = 0.f;   // M, and 2^(m - M)
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;             // heads 2 t4 and 2 t4 + 1
+        float r0 = -INFINITY, r1 = -INFINITY, w0 = INFINITY, w1 = INFINITY;  // M, and 2^(m - M)
 #pragma unroll
-        for (int i = 0; i < kStages - 1; i++) issue(i);
+        for (int i = 0; i < kStages - 1; i++) issue(i, i);
 
+        int slot = 0;
         for (int i = 0; i < mine; i++) {
             if ((i >> 5) != batch) {
                 batch++;
@@ -311,33 +341,49 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             }
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
             const float ks = __shfl_sync(0xffffffffu, ks0, i & 31), vs = __shfl_sync(0xffffffffu, vs0, i & 31);
-            const uint32_t st = ring + (i % kStages) * L::kStage;
+            __syncwarp();  // the other lanes' copies; and every lane is through with the stage before
+            const uint32_t k_from = ring + slot * L::kStage, v_from = k_from + L::kKBytes;
 
             // S^T: rows g and g + 8 are keys
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            float s[4];
+            {
+                uint32_t a[WORDS], c[WORDS];
 #pragma unroll
-            for (int j = 0; j < L::kKPer; j++) {
-                uint32_t a[L::kKVec / 4], c[L::kKVec / 4];
-                lds<L::kKVec>(a, st + (j * 32 + lane) * L::kKVec);
-                lds<L::kKVec>(c, st + ((L::kKPer + j) * 32 + lane) * L::kKVec);
+                for (int j = 0; j < L::kKPer; j++) {
+                    lds<L::kKVec>(reinterpret_cast<uint32_t(&)[L::kKVec / 4]>(a[j * (L::kKVec / 4)]), k_from + k_run(0, j));
+                    lds<L::kKVec>(reinterpret_cast<uint32_t(&)[L::kKVec / 4]>(c[j * (L::kKVec / 4)]),
+                                  k_from + k_run(1, j));
+                }
+                int d[4] = {0, 0, 0, 0};
+                auto add_digit = [&](int n) {
 #pragma unroll
-                for (int e = 0; e < L::kKVec / 4; e++) {
-                    const uint32_t wa = a[e] ^ 0x80808080u, wc = c[e] ^ 0x80808080u;
-                    const uint32_t f[4] = {codes2<false>(wa), codes2<false>(wc), codes2<true>(wa), codes2<true>(wc)};
-                    const int k = j * (L::kKVec / 4) + e;
-                    mma(s, f, qh[k][0], qh[k][1]);
-                    if constexpr (kSplit) mma(s, f, ql[k][0], ql[k][1]);
+                    for (int e = 0; e < WORDS; e += 2) mma_s8(d, a[e], c[e], a[e + 1], c[e + 1], qd[n][e], qd[n][e + 1]);
+                };
+                add_digit(0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) d[e] <<= 8;  // (128 products of 127 by 127: below 2^21)
+                add_digit(1);
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[e] = (float)d[e];
+                if constexpr (kSplit) {
+                    int d2[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int e = 0; e < WORDS; e += 2) mma_s8(d2, a[e], c[e], a[e + 1], c[e + 1], qd[DIGITS - 1][e], qd[DIGITS - 1][e + 1]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[e] = fmaf(s[e], 256.f, (float)d2[e]);
                 }
             }
-            const int key = (tile + warp + i * kWarps) * kTile + g;
-            const bool in0 = key < len, in1 = key + 8 < len;
-            const float x0 = in0 ? s[0] * (ks * fq0) : -INFINITY, x1 = in0 ? s[1] * (ks * fq1) : -INFINITY;
-            const float x2 = in1 ? s[2] * (ks * fq0) : -INFINITY, x3 = in1 ? s[3] * (ks * fq1) : -INFINITY;
+            const float g0 = ks * fq0, g1 = ks * fq1;
+            float x0 = s[0] * g0, x1 = s[1] * g1, x2 = s[2] * g0, x3 = s[3] * g1;
+            const int key = (tile + warp + i * kWarps) * kTile;
+            if (key + kTile > len) {  // the sequence's last tile
+                if (key + g >= len) x0 = x1 = -INFINITY;
+                if (key + g + 8 >= len) x2 = x3 = -INFINITY;
+            }
             const float t0 = fmaxf(x0, x2), t1 = fmaxf(x1, x3);
             // (a NaN score never moves a reference; it reaches l and O below)
-            const float lim0 = vs * w0 * ex2(t0 - m0), lim1 = vs * w1 * ex2(t1 - m1);
-            if (__any_sync(0xffffffffu, t0 > m0 + 8.f || t1 > m1 + 8.f || !(lim0 <= 256.f) || !(lim1 <= 256.f) ||
-                                           (vs > 0.f && (r0 == -INFINITY || r1 == -INFINITY)))) {
+            float v0 = vs * w0, v1 = vs * w1;  // at most 2^7, so that weights stay below 2^15
+            if (__any_sync(0xffffffffu, t0 > m0 + 8.f || t1 > m1 + 8.f || !(v0 <= 128.f) || !(v1 <= 128.f))) {
                 float c0 = t0, c1 = t1;
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) {
@@ -345,22 +391,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
                     c1 = fmaxf(c1, __shfl_xor_sync(0xffffffffu, c1, d));
                 }
                 const float lv = lg2(vs);
-                auto move = [&](float c, float& m, float& l, float& r, float& w) {
+                auto move = [&](float c, float& m, float& l, float& r, float& w, float& v) {
                     const float mn = fmaxf(m, c), rn = fmaxf(r, c + lv);
                     l *= m == mn ? 1.f : ex2(m - mn);
                     const float beta = r == rn ? 1.f : ex2(r - rn);
                     m = mn, r = rn;
-                    w = rn == -INFINITY ? 0.f : ex2(fminf(mn - rn, 127.f));
+                    w = rn == -INFINITY ? INFINITY : ex2(fminf(mn - rn, 127.f));
+                    v = vs == 0.f ? 0.f : vs * w;
                     return beta;
                 };
-                const float b0 = move(c0, m0, l0, r0, w0), b1 = move(c1, m1, l1, r1, w1);
+                const float b0 = move(c0, m0, l0, r0, w0, v0), b1 = move(c1, m1, l1, r1, w1, v1);
 #pragma unroll
                 for (int j = 0; j < MT; j++) o[j][0] *= b0, o[j][1] *= b1, o[j][2] *= b0, o[j][3] *= b1;
             }
             const float p0 = ex2(x0 - m0), p1 = ex2(x1 - m1), p2 = ex2(x2 - m0), p3 = ex2(x3 - m1);
             l0 += p0 + p2;
             l1 += p1 + p3;
-            const float v0 = vs * w0, v1 = vs * w1;
             uint32_t bh[2], bl[2];
             {
                 const float y0 = p0 * v0, y1 = p1 * v1, y2 = p2 * v0, y3 = p3 * v1;
@@ -379,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             for (int j = 0; j < L::kVPer; j++) {
                 uint32_t v[4][L::kVVec / 4];
 #pragma unroll
-                for (int r = 0; r < 4; r++) lds<L::kVVec>(v[r], st + L::kKBytes + ((r * L::kVPer + j) * 32 + lane) * L::kVVec);
+                for (int r = 0; r < 4; r++) lds<L::kVVec>(v[r], v_from + v_run(r, j));
 #pragma unroll
                 for (int e = 0; e < L::kVVec / 4; e++) {
                     // keys 2 t4 and 2 t4 + 1 (+ 8) beside one another, dims 0 1 | 2 3
@@ -398,7 +444,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
                     }
                 }
             }
-            issue(i + kStages - 1);
+            issue(i + kStages - 1, slot == 0 ? kStages - 1 : slot - 1);
+            slot = slot == kStages - 1 ? 0 : slot + 1;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
