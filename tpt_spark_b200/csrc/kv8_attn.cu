@@ -38,9 +38,10 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kStages = 3;
-constexpr int kCtasPerSm = 4;
+constexpr int kCtasPerSm = 3;  // (4 of 128 registers: 99 us for 8 sequences of 32k against 93)
 constexpr int kTile = 16;       // keys
 constexpr int kHeads = 8;       // query heads per pass over the keys (columns of the products)
+constexpr int kBlock = 128;     // parts whose weights are in shared memory at a time
 constexpr int kMinTiles = 16;   // tiles that make a CTA worth its share of the join
 
 template <int HD>
@@ -53,8 +54,10 @@ struct Lay {
     static constexpr int kStage = 2 * kKBytes;
     static constexpr int kRing = kWarps * kStages * kStage;
     static constexpr int kRecord = 3 * kHeads + kHeads * HD;  // floats: m, l, M, O of one part
-    static constexpr int kJoin = kWarps * kRecord * 4;
-    static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+    // the warps' records, later the weights of a block of parts and their references
+    static constexpr int kJoinA = kWarps * kRecord * 4, kJoinB = (2 * kBlock * kHeads + kThreads * 2) * 4;
+    static constexpr int kJoin = kJoinA > kJoinB ? kJoinA : kJoinB;
+    static constexpr int kSmem = kRing + kJoin;
 };
 
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
@@ -110,15 +113,15 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
 }
 
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&x)[4]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(p));
-        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-    } else {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-        const T *a = reinterpret_cast<const T*>(&v.x), *b = reinterpret_cast<const T*>(&v.y);
-        x[0] = to_f32(a[0]), x[1] = to_f32(a[1]), x[2] = to_f32(b[0]), x[3] = to_f32(b[1]);
-    }
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(a, b), pack2<T>(c, d));
+}
+
+// a / b of numbers that are not negative; 32-bit where both fit.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+    return a / b;
 }
 
 struct Params {
@@ -173,10 +176,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             for (int i = tid; i < p.n_heads * HD; i += kThreads)
                 static_cast<T*>(p.out)[(int64_t)b * p.n_heads * HD + i] = static_cast<T>(0.f);
     total *= pairs;
-    const int64_t ctas = min((int64_t)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
-    if (blockIdx.x >= ctas) return;
-    int64_t at = blockIdx.x * total / ctas;
-    const int64_t end = (blockIdx.x + 1) * total / ctas, first = at;
+    const int ctas = (int)min((int64_t)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
+    if ((int)blockIdx.x >= ctas) return;
+    // CTA c begins at c share + min(c, more)
+    const int64_t share = quotient(total, ctas);
+    const int more = (int)(total - share * ctas);
+    auto begins = [&](int c) { return c * share + min(c, more); };
+    auto cta_of = [&](int64_t t) {  // whose range holds tile t
+        const int64_t split = (share + 1) * more;
+        return t < split ? (int)quotient(t, share + 1) : more + (int)quotient(t - split, share);
+    };
+    int64_t at = begins(blockIdx.x);
+    const int64_t end = begins(blockIdx.x + 1), first = at;
     {
         int64_t before = 0;  // tiles before the block of sequences
         bool found = false;
@@ -199,8 +210,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             const bool mine = t > 0 && lo <= at && at < hi;
             if (mine) {
                 s_start[0] = b;
-                s_start[1] = (int)((at - lo) / t);
-                s_start[2] = (int)((at - lo) % t);
+                s_start[1] = (int)quotient(at - lo, t);
+                s_start[2] = (int)(at - lo) - s_start[1] * t;
             }
             found = __syncthreads_or(mine);
             for (int w = 0; w < kWarps; w++) before += s_scan[w];
@@ -231,107 +242,131 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
     auto v_run = [&](int r, int j) {
         return (r >> 1) * 8 * HD + (HD == 64 ? v_of ^ ((r & 1) * 64) : v_of + (r & 1) * HD + j * L::kVVec);
     };
-    for (; at < end;) {
-        const int n = (int)min((int64_t)(tiles - tile), end - at);  // tiles of this piece
-        const int kvh = pair / subs, h0 = kvh * G + (pair % subs) * kHeads, nh = min(kHeads, kvh * G + G - h0);
 
+    float* rec = reinterpret_cast<float*>(smem + L::kRing);  // the joins' memory
+    auto ratio = [](float a, float m) { return a == m ? 1.f : ex2(a - m); };
+
+    // ---- a piece: the CTA's part of one pair's tiles
+    int n, kvh, h0, nh, mine;  // its tiles; heads; tiles of this warp
+    int id0, id1, batch;       // page ids and scales: lane i holds those of the warp's tile 32 batch + i, and of the next batch
+    float ks0, vs0, ks1, vs1;
+    const int8_t *k_at, *v_at;
+    constexpr int WORDS = HD / 16;  // of four dims
+    using Four = typename std::conditional<kSplit, float4, uint2>::type;
+    Four q_raw[WORDS];
+    const int page_mask = p.c.page - 1;
+    const int64_t page_bytes = (int64_t)p.c.n_kv * p.c.page * HD;  // of all heads
+    auto fetch = [&](int of, int& id, float& ks, float& vs) {
+        const int i = 32 * of + lane;
+        id = 0;
+        ks = vs = 0.f;
+        if (i < mine) {
+            const int pos = (tile + warp + i * kWarps) * kTile;
+            id = p.c.table[(int64_t)b * p.c.max_pages + pos / p.c.page];
+            if (id >= 0 && id < p.c.n_pages) {
+                const int64_t k = (int64_t)id * p.c.n_kv + kvh;
+                ks = p.c.k_scale[k];
+                vs = p.c.v_scale[k];
+            } else {  // not in the cache: not followed
+                if (p.c.status) atomicExch(p.c.status, TPTC_ERR_ARG);
+                id = 0;
+                ks = vs = __int_as_float(0x7fc00000);
+            }
+        }
+    };
+    auto issue = [&](int i, int slot) {  // 2 x 16 rows, each a run of the page
+        if (i < mine) {
+            const int id = __shfl_sync(0xffffffffu, (i >> 5) == batch ? id0 : id1, i & 31);
+            const int64_t off = id * page_bytes + (((tile + warp + i * kWarps) * kTile) & page_mask) * HD;
+            const int8_t *k = k_at + off, *v = v_at + off;
+            const uint32_t kd = ring + slot * L::kStage, vd = kd + L::kKBytes;
+#pragma unroll
+            for (int e = 0; e < HD / 32; e++) {
+                copy_async(kd + e * 512 + k_to, k + e * 512);
+                copy_async(vd + e * 512 + (HD == 128 && (e & 1) ? v_to ^ 64 : v_to), v + e * 512);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto begin = [&] {  // everything of it that can be on its way
+        n = (int)min((int64_t)(tiles - tile), end - at);
+        kvh = pair / subs;
+        h0 = kvh * G + (pair % subs) * kHeads;
+        nh = min(kHeads, kvh * G + G - h0);
+        mine = n > warp ? (n - warp + kWarps - 1) / kWarps : 0;
+        batch = 0;
+        fetch(0, id0, ks0, vs0);
+        fetch(1, id1, ks1, vs1);
+        k_at = p.c.k + (int64_t)kvh * p.c.page * HD + lane * 16;
+        v_at = p.c.v + (int64_t)kvh * p.c.page * HD + lane * 16;
+        const T* q = static_cast<const T*>(p.q) + (int64_t)b * p.q_stride + (int64_t)(h0 + g) * HD;
+#pragma unroll
+        for (int w = 0; w < WORDS; w++) {
+            constexpr int per = L::kKVec / 4;  // words per run
+            q_raw[w] = Four{};
+            if (g < nh) q_raw[w] = __ldg(reinterpret_cast<const Four*>(q + (w / per) * (4 * L::kKVec) + t4 * L::kKVec + (w % per) * 4));
+        }
+#pragma unroll
+        for (int i = 0; i < kStages - 1; i++) issue(i, i);
+    };
+
+    begin();
+    for (;;) {
         // ---- the queries, as the B operand: thread holds the digits of head g, dims of its own bytes of K
-        constexpr int DIGITS = kSplit ? 3 : 2, WORDS = HD / 16;  // words of four dims
+        constexpr int DIGITS = kSplit ? 3 : 2;
         uint32_t qd[DIGITS][WORDS];
         float fq0, fq1;
         {
-            const T* q = static_cast<const T*>(p.q) + (int64_t)b * p.q_stride + (int64_t)(h0 + g) * HD;
             float x[WORDS][4], top = 0.f;
 #pragma unroll
-            for (int s = 0; s < WORDS; s++) {
-                constexpr int per = L::kKVec / 4;  // words per copy
-                const int d = (s / per) * (4 * L::kKVec) + t4 * L::kKVec + (s % per) * 4;
-                x[s][0] = x[s][1] = x[s][2] = x[s][3] = 0.f;
-                if (g < nh) load4(q + d, x[s]);
+            for (int w = 0; w < WORDS; w++) {
+                const T* raw = reinterpret_cast<const T*>(&q_raw[w]);
 #pragma unroll
-                for (int e = 0; e < 4; e++) top = fmaxf(top, x[s][e] == x[s][e] ? fabsf(x[s][e]) : INFINITY);
+                for (int e = 0; e < 4; e++) {
+                    x[w][e] = to_f32(raw[e]);
+                    top = fmaxf(top, x[w][e] == x[w][e] ? fabsf(x[w][e]) : INFINITY);
+                }
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // the largest element becomes 127 in its highest digit (a power of two first, so that no factor
             // leaves f32's range); an element that is not finite makes the head's scores NaN
-            const int e2 = top < 1.17549435e-38f ? -126 : (int)(__float_as_uint(top) >> 23) - 126;
+            const int e2 = max(-126, min(126, (int)(__float_as_uint(top) >> 23) - 126));
             constexpr float kMost = kSplit ? 127.f * 65536.f : 127.f * 256.f;
-            const float down = ldexpf(1.f, -e2), unit = top * down, up = unit > 0.f ? kMost / unit : 0.f;
+            const float down = __uint_as_float((uint32_t)(127 - e2) << 23), unit = top * down;
+            const float up = unit > 0.f ? __fdividef(kMost, unit) : 0.f;
 #pragma unroll
             for (int s = 0; s < WORDS; s++) {
+                uint32_t v[4];
+                auto pack = [&](uint32_t byte) {  // byte 0 or 1 of each
+                    const uint32_t sel = byte | (byte + 4) << 4;
+                    return __byte_perm(__byte_perm(v[0], v[1], sel), __byte_perm(v[2], v[3], sel), 0x5410);
+                };
 #pragma unroll
-                for (int d = 0; d < DIGITS; d++) qd[d][s] = 0;
+                for (int e = 0; e < 4; e++) v[e] = (uint32_t)__float2int_rn(x[s][e] * down * up);
+                qd[DIGITS - 1][s] = pack(0);
+                // the next digit is signed as well: (v - digit) / 256 = (v + 128) >> 8
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    int v = __float2int_rn(x[s][e] * down * up);
+                for (int d = DIGITS - 2; d >= 0; d--) {
 #pragma unroll
-                    for (int d = DIGITS - 1; d >= 0; d--) {  // signed digits: the carry goes on
-                        const int low = d ? (int)(int8_t)v : v;
-                        v = (v - low) >> 8;
-                        qd[d][s] |= (uint32_t)(low & 255) << (8 * e);
-                    }
+                    for (int e = 0; e < 4; e++) v[e] += 128;
+                    qd[d][s] = pack(1);
+                    if (d > 0)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[e] = (uint32_t)((int)v[e] >> 8);
                 }
             }
-            const float f = top <= 3.402823466e38f ? ldexpf(p.scale_log2 * (unit / kMost), e2) : __int_as_float(0x7fc00000);
+            const float f = top <= 3.402823466e38f ? p.scale_log2 * (unit * (1.f / kMost)) * __uint_as_float((uint32_t)(127 + e2) << 23)
+                                                   : __int_as_float(0x7fc00000);
             fq0 = __shfl_sync(0xffffffffu, f, 8 * t4);
             fq1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
         }
-
-        // ---- page ids and scales: lane i holds those of this warp's tile 32 * batch + i
-        const int mine = n > warp ? (n - warp + kWarps - 1) / kWarps : 0;  // tiles of this warp
-        const int32_t* table = p.c.table + (int64_t)b * p.c.max_pages;
-        auto fetch = [&](int batch, int& id, float& ks, float& vs) {
-            const int i = 32 * batch + lane;
-            id = 0;
-            ks = vs = 0.f;
-            if (i < mine) {
-                const int64_t pos = (int64_t)(tile + warp + i * kWarps) * kTile;
-                id = table[pos / p.c.page];
-                if (id >= 0 && id < p.c.n_pages) {
-                    const int64_t k = (int64_t)id * p.c.n_kv + kvh;
-                    ks = p.c.k_scale[k];
-                    vs = p.c.v_scale[k];
-                } else {  // not in the cache: not followed
-                    if (p.c.status) atomicExch(p.c.status, TPTC_ERR_ARG);
-                    id = 0;
-                    ks = vs = __int_as_float(0x7fc00000);
-                }
-            }
-        };
-        int id0, id1;
-        float ks0, vs0, ks1, vs1;
-        fetch(0, id0, ks0, vs0);
-        fetch(1, id1, ks1, vs1);
-        int batch = 0;  // id0 .. are of this batch, id1 .. of the next
-
-        const int page_mask = p.c.page - 1;
-        const int64_t page_bytes = (int64_t)p.c.n_kv * p.c.page * HD;  // of all heads
-        const int8_t* k_at = p.c.k + (int64_t)kvh * p.c.page * HD + lane * 16;
-        const int8_t* v_at = p.c.v + (int64_t)kvh * p.c.page * HD + lane * 16;
-        auto issue = [&](int i, int slot) {  // 2 x 16 rows, each a run of the page
-            if (i < mine) {
-                const int id = __shfl_sync(0xffffffffu, (i >> 5) == batch ? id0 : id1, i & 31);
-                const int64_t off = id * page_bytes + (((tile + warp + i * kWarps) * kTile) & page_mask) * HD;
-                const int8_t *k = k_at + off, *v = v_at + off;
-                const uint32_t kd = ring + slot * L::kStage, vd = kd + L::kKBytes;
-#pragma unroll
-                for (int n = 0; n < HD / 32; n++) {
-                    copy_async(kd + n * 512 + k_to, k + n * 512);
-                    copy_async(vd + n * 512 + (HD == 128 && (n & 1) ? v_to ^ 64 : v_to), v + n * 512);
-                }
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
 
         float o[MT][4];
 #pragma unroll
         for (int j = 0; j < MT; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;             // heads 2 t4 and 2 t4 + 1
         float r0 = -INFINITY, r1 = -INFINITY, w0 = INFINITY, w1 = INFINITY;  // M, and 2^(m - M)
-#pragma unroll
-        for (int i = 0; i < kStages - 1; i++) issue(i, i);
-
         int slot = 0;
         for (int i = 0; i < mine; i++) {
             if ((i >> 5) != batch) {
@@ -354,23 +389,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
                     lds<L::kKVec>(reinterpret_cast<uint32_t(&)[L::kKVec / 4]>(c[j * (L::kKVec / 4)]),
                                   k_from + k_run(1, j));
                 }
-                int d[4] = {0, 0, 0, 0};
-                auto add_digit = [&](int n) {
+                // (a chain of products for each digit: they run side by side; 128 products of 127 by 127 are below 2^21)
+                int d[DIGITS][4];
 #pragma unroll
-                    for (int e = 0; e < WORDS; e += 2) mma_s8(d, a[e], c[e], a[e + 1], c[e + 1], qd[n][e], qd[n][e + 1]);
-                };
-                add_digit(0);
+                for (int n = 0; n < DIGITS; n++) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0;
 #pragma unroll
-                for (int e = 0; e < 4; e++) d[e] <<= 8;  // (128 products of 127 by 127: below 2^21)
-                add_digit(1);
+                for (int e = 0; e < WORDS; e += 2)
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[e] = (float)d[e];
-                if constexpr (kSplit) {
-                    int d2[4] = {0, 0, 0, 0};
+                    for (int n = 0; n < DIGITS; n++) mma_s8(d[n], a[e], c[e], a[e + 1], c[e + 1], qd[n][e], qd[n][e + 1]);
 #pragma unroll
-                    for (int e = 0; e < WORDS; e += 2) mma_s8(d2, a[e], c[e], a[e + 1], c[e + 1], qd[DIGITS - 1][e], qd[DIGITS - 1][e + 1]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[e] = fmaf(s[e], 256.f, (float)d2[e]);
+                for (int e = 0; e < 4; e++) {
+                    s[e] = (float)(d[0][e] * 256 + d[1][e]);
+                    if constexpr (kSplit) s[e] = fmaf(s[e], 256.f, (float)d[DIGITS - 1][e]);
                 }
             }
             const float g0 = ks * fq0, g1 = ks * fq1;
@@ -447,16 +477,33 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             issue(i + kStages - 1, slot == 0 ? kStages - 1 : slot - 1);
             slot = slot == kStages - 1 ? 0 : slot + 1;
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
             l0 += __shfl_xor_sync(0xffffffffu, l0, d);
             l1 += __shfl_xor_sync(0xffffffffu, l1, d);
         }
-        __syncthreads();  // the ring becomes the join's memory
+
+        // ---- the next piece's copies run under this one's join
+        const int was_n = n, was_h = nh, was_tiles = tiles;
+        const int64_t piece0 = at - tile, piece1 = piece0 + tiles;  // the pair's part of the line
+        T* out = static_cast<T*>(p.out) + ((int64_t)b * p.n_heads + h0) * HD;
+        int* counter = p.counters + (int64_t)b * pairs + pair;
+        at += n;
+        const bool again = at < end;
+        if (again) {
+            tile = 0;
+            if (++pair == pairs) {
+                pair = 0;
+                do len = length_of(p, ++b, false);
+                while (len == 0);  // (a sequence with tiles follows: the range goes on)
+                tiles = (len + kTile - 1) / kTile;
+            }
+            __syncwarp();  // every lane is through with the ring
+            begin();
+        }
 
         // ---- join the warps
-        float* rec = reinterpret_cast<float*>(smem);
+        __syncthreads();  // the last join's memory is free
         {
             float* me = rec + warp * L::kRecord;
             if (g == 0) {
@@ -473,15 +520,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             }
         }
         __syncthreads();
-        const bool whole = n == tiles;
-        const int64_t piece0 = at - tile, piece1 = piece0 + tiles;  // the pair's part of the line
+        const bool whole = was_n == was_tiles;
         // slot 0 of the CTA: a pair that began before its range; 1: one that begins inside it
         float* out_rec = p.records + (int64_t)(2 * blockIdx.x + (first >= piece0 ? 0 : 1)) * L::kRecord;
-        T* out = static_cast<T*>(p.out) + ((int64_t)b * p.n_heads + h0) * HD;
-
-        // out[h][d..] of `parts` records of rec(i), each scaled to the largest references; thread
-        // tid holds four dims of a head per step
-        auto ratio = [](float a, float m) { return a == m ? 1.f : ex2(a - m); };
+        // a thread holds four dims of a head per step; parts are scaled to the largest references
         for (int i = tid; i < kHeads * (HD / 4); i += kThreads) {
             const int h = i / (HD / 4), d = (i % (HD / 4)) * 4;
             float m = -INFINITY, r = -INFINITY;
@@ -494,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
 #pragma unroll
             for (int w = 0; w < kWarps; w++) {
                 const float* a = rec + w * L::kRecord;
-                if (w >= n) break;  // a warp without a tile
+                if (w >= was_n) break;  // a warp without a tile
                 l += a[kHeads + h] * ratio(a[h], m);
                 const float f = ratio(a[2 * kHeads + h], r);
                 const float4 v = *reinterpret_cast<const float4*>(a + 3 * kHeads + h * HD + d);
@@ -502,68 +544,86 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             }
             if (whole) {
                 const float f = (r == -INFINITY ? 0.f : ex2(r - m)) / l;
-                if (h < nh)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) out[h * HD + d + e] = static_cast<T>(y[e] * f);
+                if (h < was_h) store4(out + h * HD + d, y[0] * f, y[1] * f, y[2] * f, y[3] * f);
             } else {
                 if (d == 0) out_rec[h] = m, out_rec[kHeads + h] = l, out_rec[2 * kHeads + h] = r;
                 *reinterpret_cast<float4*>(out_rec + 3 * kHeads + h * HD + d) = make_float4(y[0], y[1], y[2], y[3]);
             }
         }
         if (!whole) {
-            const int64_t c0 = ((piece0 + 1) * ctas - 1) / total, c1 = (piece1 * ctas - 1) / total;
-            const int parts = (int)(c1 - c0 + 1);
-            int* counter = p.counters + (int64_t)b * pairs + pair;
-            __threadfence();
+            const int c0 = cta_of(piece0), c1 = cta_of(piece1 - 1), parts = c1 - c0 + 1;
             __syncthreads();
-            if (tid == 0) {
-                s_last = atomicAdd(counter, 1) == parts - 1;
+            if (tid == 0) {  // the release covers this CTA's record, the last one's acquire all of them
+                int n_before;
+                asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(n_before) : "l"(counter) : "memory");
+                s_last = n_before == parts - 1;
                 if (s_last) *counter = 0;
-                __threadfence();
             }
             __syncthreads();
             if (s_last) {
                 auto part = [&](int i) {
-                    const int64_t c = c0 + i;
-                    return p.records + (2 * c + (c * total / ctas >= piece0 ? 0 : 1)) * L::kRecord;
+                    const int c = c0 + i;
+                    return p.records + (2 * (int64_t)c + (begins(c) >= piece0 ? 0 : 1)) * L::kRecord;
                 };
-                for (int i = tid; i < kHeads * (HD / 4); i += kThreads) {
-                    const int h = i / (HD / 4), d = (i % (HD / 4)) * 4;
-                    if (h >= nh) continue;
+                // the references of all parts, 16 parts of 8 heads at a time
+                constexpr int kRows = kThreads / kHeads;
+                float *w_l = rec, *w_o = rec + kBlock * kHeads, *ref = rec + 2 * kBlock * kHeads;
+                const int h8 = tid % kHeads, k8 = tid / kHeads;
+                {
                     float m = -INFINITY, r = -INFINITY;
-                    for (int k = 0; k < parts; k++) {
-                        const float* a = part(k);
-                        m = fmaxf(m, __ldcg(a + h));
-                        r = fmaxf(r, __ldcg(a + 2 * kHeads + h));
-                    }
-                    float l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-                    for (int k = 0; k < parts; k++) {
+                    for (int k = k8; k < parts; k += kRows) {
                         const float* a = part(k);
-                        l += __ldcg(a + kHeads + h) * ratio(__ldcg(a + h), m);
-                        const float f = ratio(__ldcg(a + 2 * kHeads + h), r);
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(a + 3 * kHeads + h * HD + d));
-                        y[0] += v.x * f, y[1] += v.y * f, y[2] += v.z * f, y[3] += v.w * f;
+                        m = fmaxf(m, __ldcg(a + h8));
+                        r = fmaxf(r, __ldcg(a + 2 * kHeads + h8));
                     }
-                    const float f = (r == -INFINITY ? 0.f : ex2(r - m)) / l;
+                    ref[k8 * 2 * kHeads + h8] = m;
+                    ref[k8 * 2 * kHeads + kHeads + h8] = r;
+                }
+                __syncthreads();
+                float m_all = -INFINITY, r_all = -INFINITY;  // of head h8
+                for (int k = 0; k < kRows; k++) {
+                    m_all = fmaxf(m_all, ref[k * 2 * kHeads + h8]);
+                    r_all = fmaxf(r_all, ref[k * 2 * kHeads + kHeads + h8]);
+                }
+                constexpr int kSteps = (kHeads * (HD / 4) + kThreads - 1) / kThreads;
+                float l[kSteps], y[kSteps][4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) out[h * HD + d + e] = static_cast<T>(y[e] * f);
+                for (int e = 0; e < kSteps; e++) l[e] = y[e][0] = y[e][1] = y[e][2] = y[e][3] = 0.f;
+                for (int k0 = 0; k0 < parts; k0 += kBlock) {
+                    const int count = min(kBlock, parts - k0);
+                    __syncthreads();
+                    for (int k = k8; k < count; k += kRows) {
+                        const float* a = part(k0 + k);
+                        w_l[k * kHeads + h8] = __ldcg(a + kHeads + h8) * ratio(__ldcg(a + h8), m_all);
+                        w_o[k * kHeads + h8] = ratio(__ldcg(a + 2 * kHeads + h8), r_all);
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int e = 0; e < kSteps; e++) {
+                        const int i = tid + e * kThreads, h = i / (HD / 4), d = (i % (HD / 4)) * 4;
+                        if (h >= was_h) continue;
+#pragma unroll 8
+                        for (int k = 0; k < count; k++) {
+                            const float f = w_o[k * kHeads + h];
+                            const float4 v = __ldcg(reinterpret_cast<const float4*>(part(k0 + k) + 3 * kHeads + h * HD + d));
+                            l[e] += w_l[k * kHeads + h];
+                            y[e][0] += v.x * f, y[e][1] += v.y * f, y[e][2] += v.z * f, y[e][3] += v.w * f;
+                        }
+                    }
+                }
+                if (k8 == 0) ref[h8] = r_all == -INFINITY ? 0.f : ex2(r_all - m_all);
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < kSteps; e++) {
+                    const int i = tid + e * kThreads, h = i / (HD / 4), d = (i % (HD / 4)) * 4;
+                    if (h >= was_h) continue;
+                    const float f = ref[h] / l[e];
+                    store4(out + h * HD + d, y[e][0] * f, y[e][1] * f, y[e][2] * f, y[e][3] * f);
                 }
             }
         }
-        __syncthreads();  // the join's memory becomes the ring again
-
-        // ---- the next pair
-        at += n;
-        tile = 0;
-        if (++pair == pairs) {
-            pair = 0;
-            do {
-                if (++b >= p.c.n_seq) break;
-                len = length_of(p, b, false);
-            } while (len == 0);
-            tiles = (len + kTile - 1) / kTile;
-        }
+        if (!again) break;
     }
 }
 
