@@ -42,7 +42,10 @@ constexpr int kCtasPerSm = 3;  // (4 of 128 registers: 99 us for 8 sequences of 
 constexpr int kTile = 16;       // keys
 constexpr int kHeads = 8;       // query heads per pass over the keys (columns of the products)
 constexpr int kBlock = 128;     // parts whose weights are in shared memory at a time
-constexpr int kMinTiles = 16;   // tiles that make a CTA worth its share of the join
+constexpr int kMinTiles = 16;   // units that make a CTA worth its share of the join
+// A pair's place on the line: kSetup units for its queries and its join, then its tiles.  (With tiles alone, ranges
+// of many short sequences took longest: 69 us instead of 56 for 32 sequences of 40 to 8000 positions.)
+constexpr int kSetup = 16;
 
 template <int HD>
 struct Lay {
@@ -157,14 +160,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int G = p.n_heads / p.c.n_kv, subs = (G + kHeads - 1) / kHeads, pairs = p.c.n_kv * subs;
 
-    // ---- this CTA's range of the line of tiles
-    auto tiles_of = [&](int b, bool report) {
-        return b < p.c.n_seq ? (length_of(p, b, report) + kTile - 1) / kTile : 0;
+    // ---- this CTA's range of the line
+    auto units_of = [&](int b, bool report) {
+        const int t = b < p.c.n_seq ? (length_of(p, b, report) + kTile - 1) / kTile : 0;
+        return t ? t + kSetup : 0;
     };
-    const int tiles0 = tiles_of(tid, blockIdx.x == 0);  // of the first kThreads sequences
+    const int units0 = units_of(tid, blockIdx.x == 0);  // of the first kThreads sequences
     int64_t total = 0;
     for (int b0 = 0; b0 < p.c.n_seq; b0 += kThreads) {
-        const int t = warp_sum_i(b0 == 0 ? tiles0 : tiles_of(b0 + tid, blockIdx.x == 0));
+        const int t = warp_sum_i(b0 == 0 ? units0 : units_of(b0 + tid, blockIdx.x == 0));
         if (b0 > 0) __syncthreads();
         if (lane == 0) s_scan[warp] = t;
         __syncthreads();
@@ -182,17 +186,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
     const int64_t share = quotient(total, ctas);
     const int more = (int)(total - share * ctas);
     auto begins = [&](int c) { return c * share + min(c, more); };
-    auto cta_of = [&](int64_t t) {  // whose range holds tile t
+    auto cta_of = [&](int64_t t) {  // whose range holds unit t
         const int64_t split = (share + 1) * more;
         return t < split ? (int)quotient(t, share + 1) : more + (int)quotient(t - split, share);
     };
-    int64_t at = begins(blockIdx.x);
-    const int64_t end = begins(blockIdx.x + 1), first = at;
+    const int64_t first = begins(blockIdx.x), end = begins(blockIdx.x + 1);
     {
-        int64_t before = 0;  // tiles before the block of sequences
+        int64_t before = 0;  // units before the block of sequences
         bool found = false;
         for (int b0 = 0; b0 < p.c.n_seq && !found; b0 += kThreads) {
-            const int b = b0 + tid, t = b0 == 0 ? tiles0 : tiles_of(b, false);
+            const int b = b0 + tid, t = b0 == 0 ? units0 : units_of(b, false);
             int incl = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -207,18 +210,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             int64_t lead = before;
             for (int w = 0; w < warp; w++) lead += s_scan[w];
             const int64_t lo = (lead + incl - t) * pairs, hi = (lead + incl) * pairs;
-            const bool mine = t > 0 && lo <= at && at < hi;
+            const bool mine = t > 0 && lo <= first && first < hi;
             if (mine) {
                 s_start[0] = b;
-                s_start[1] = (int)quotient(at - lo, t);
-                s_start[2] = (int)(at - lo) - s_start[1] * t;
+                s_start[1] = (int)quotient(first - lo, t);
+                s_start[2] = (int)(first - lo) - s_start[1] * t;
             }
             found = __syncthreads_or(mine);
             for (int w = 0; w < kWarps; w++) before += s_scan[w];
         }
     }
-    int b = s_start[0], pair = s_start[1], tile = s_start[2];
+    int b = s_start[0], pair = s_start[1], tile = max(0, s_start[2] - kSetup);
     int len = length_of(p, b, false), tiles = (len + kTile - 1) / kTile;
+    int64_t piece0 = first - s_start[2];  // the pair's first unit
+    if (end - piece0 <= kSetup) return;   // not a tile
 
     const uint32_t ring = smem_u32(smem) + warp * (kStages * L::kStage);
     // Where a lane's copies go in a stage (512 bytes per copy of the warp, rows in order), and where a thread
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     auto begin = [&] {  // everything of it that can be on its way
-        n = (int)min((int64_t)(tiles - tile), end - at);
+        n = (int)min((int64_t)tiles, end - piece0 - kSetup) - tile;
         kvh = pair / subs;
         h0 = kvh * G + (pair % subs) * kHeads;
         nh = min(kHeads, kvh * G + G - h0);
@@ -485,12 +490,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
 
         // ---- the next piece's copies run under this one's join
         const int was_n = n, was_h = nh, was_tiles = tiles;
-        const int64_t piece0 = at - tile, piece1 = piece0 + tiles;  // the pair's part of the line
+        const int64_t was0 = piece0, was1 = piece0 + kSetup + tiles;  // the pair's part of the line
         T* out = static_cast<T*>(p.out) + ((int64_t)b * p.n_heads + h0) * HD;
         int* counter = p.counters + (int64_t)b * pairs + pair;
-        at += n;
-        const bool again = at < end;
+        const bool again = end - was1 > kSetup;
         if (again) {
+            piece0 = was1;
             tile = 0;
             if (++pair == pairs) {
                 pair = 0;
@@ -522,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
         __syncthreads();
         const bool whole = was_n == was_tiles;
         // slot 0 of the CTA: a pair that began before its range; 1: one that begins inside it
-        float* out_rec = p.records + (int64_t)(2 * blockIdx.x + (first >= piece0 ? 0 : 1)) * L::kRecord;
+        float* out_rec = p.records + (int64_t)(2 * blockIdx.x + (first >= was0 ? 0 : 1)) * L::kRecord;
         // a thread holds four dims of a head per step; parts are scaled to the largest references
         for (int i = tid; i < kHeads * (HD / 4); i += kThreads) {
             const int h = i / (HD / 4), d = (i % (HD / 4)) * 4;
@@ -551,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             }
         }
         if (!whole) {
-            const int c0 = cta_of(piece0), c1 = cta_of(piece1 - 1), parts = c1 - c0 + 1;
+            const int c0 = cta_of(was0 + kSetup), c1 = cta_of(was1 - 1), parts = c1 - c0 + 1;
             __syncthreads();
             if (tid == 0) {  // the release covers this CTA's record, the last one's acquire all of them
                 int n_before;
@@ -563,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             if (s_last) {
                 auto part = [&](int i) {
                     const int c = c0 + i;
-                    return p.records + (2 * (int64_t)c + (begins(c) >= piece0 ? 0 : 1)) * L::kRecord;
+                    return p.records + (2 * (int64_t)c + (begins(c) >= was0 ? 0 : 1)) * L::kRecord;
                 };
                 // the references of all parts, 16 parts of 8 heads at a time
                 constexpr int kRows = kThreads / kHeads;
