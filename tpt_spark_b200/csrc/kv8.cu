@@ -8,7 +8,8 @@
 // touched page, kv head), which keeps the page's rotated rows in registers between the maximum
 // and the rounding (each input is read once).  A second CTA beside it rotates the query rows of
 // its head group and positions, four heads of a token per thread with one pair of cos and sin vectors, so one launch moves q, k and
-// v.  Bound by HBM for prompts and by launch latency for decode steps: APPTIME.
+// v.  Bound by HBM for prompts and by launch latency for
+// decode steps: 44 us for 7900 bf16 tokens of 32 heads on 8 (194 MB, 4.4 TB/s), 6.6 us for one token of each of 64 sequences.
 #include <algorithm>
 
 #include "serve.h"
@@ -151,7 +152,8 @@ __device__ __forceinline__ void rescale_codes(int8_t* codes, int n, float ratio)
 
 // NR: passes of the CTA over a page's rows (16 or 32 rows each).
 template <typename T, int HD, int NR>
-__global__ void __launch_bounds__(kThreads) kv8_append_kernel(const __grid_constant__ Kv8Append p) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : NR == 4 ? 3 : 4)
+    kv8_append_kernel(const __grid_constant__ Kv8Append p) {
     constexpr int GS = HD == 64 ? 8 : 16;  // lanes per row (12 of 16 work at head_dim 96)
     constexpr int RP = kThreads / GS;
     __shared__ float s_top[2][kThreads / 32];
@@ -287,10 +289,12 @@ __device__ __forceinline__ void store_values(T* dst, const uint4& w, float scale
     store8(dst + 8, x[1]);
 }
 
-// One CTA per (sequence, page, group of kv heads): 16 codes per thread and load, a page's rows of
-// one head contiguous, so that loads and stores both run along head_dim.
+// One CTA per (sequence, page, group of kv heads): 16 codes per load, kReadLoads of K and of V in flight per
+// thread; a page's rows of one head are contiguous, so that loads and stores both run along head_dim.  HBM bound:
+// 28 us for 21k positions of 8 heads of 128 (130 MB, 4.6 TB/s; 5.8 TB/s for ten times that), 3.7 us for 300.
+constexpr int kReadLoads = 2;  // (and 5 CTAs per SM: 255 us for 240k positions, 298 with 4 loads and 3 CTAs)
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constant__ Kv8Read p) {
+__global__ void __launch_bounds__(kThreads, 5) kv8_read_kernel(const __grid_constant__ Kv8Read p) {
     constexpr int CH = HD / 16;
     const int groups = (p.c.n_kv + p.heads_per_cta - 1) / p.heads_per_cta;
     const int g = blockIdx.x % groups, unit = blockIdx.x / groups, u = unit % p.units, b = unit / p.units;
@@ -299,20 +303,28 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const __grid_constan
     const int page_id = p.c.table[s.entry];
     if (!in_cache(p.c, page_id)) return;
     const int h0 = g * p.heads_per_cta, heads = min(p.heads_per_cta, p.c.n_kv - h0);
-    const int per = s.n * CH, total = heads * per;
-#pragma unroll 2
-    for (int i = threadIdx.x; i < total; i += kThreads) {
-        const int hh = i / per, rem = i - hh * per, row = rem / CH, ch = rem - row * CH;
-        const int64_t at = (int64_t)page_id * p.c.n_kv + h0 + hh;
-        const int64_t src = (at * p.c.page + s.off + row) * HD + ch * 16;
-        const int64_t dst = ((int64_t)(s.first + row) * p.c.n_kv + h0 + hh) * HD + ch * 16;
-        if (p.k_out) {
-            const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p.c.k + src));
-            store_values(static_cast<T*>(p.k_out) + dst, w, p.c.k_scale[at]);
+    const int64_t at = (int64_t)page_id * p.c.n_kv + h0;
+    const int8_t *k = p.c.k + at * p.c.page * HD, *v = p.c.v + at * p.c.page * HD;
+    const int shift = 31 - __clz(p.c.page), total = heads * p.c.page * CH;
+    for (int i0 = 0; i0 < total; i0 += kReadLoads * kThreads) {
+        uint4 wk[kReadLoads], wv[kReadLoads];
+        float sk[kReadLoads], sv[kReadLoads];
+        int64_t dst[kReadLoads];
+#pragma unroll
+        for (int e = 0; e < kReadLoads; e++) {
+            const int i = i0 + e * kThreads + threadIdx.x, r = i / CH, hh = r >> shift, row = (r & (p.c.page - 1)) - s.off;
+            dst[e] = i < total && row >= 0 && row < s.n
+                         ? ((int64_t)(s.first + row) * p.c.n_kv + h0 + hh) * HD + (i - r * CH) * 16
+                         : -1;
+            if (dst[e] < 0) continue;
+            if (p.k_out) wk[e] = __ldcs(reinterpret_cast<const uint4*>(k) + i), sk[e] = p.c.k_scale[at + hh];
+            if (p.v_out) wv[e] = __ldcs(reinterpret_cast<const uint4*>(v) + i), sv[e] = p.c.v_scale[at + hh];
         }
-        if (p.v_out) {
-            const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p.c.v + src));
-            store_values(static_cast<T*>(p.v_out) + dst, w, p.c.v_scale[at]);
+#pragma unroll
+        for (int e = 0; e < kReadLoads; e++) {
+            if (dst[e] < 0) continue;
+            if (p.k_out) store_values(static_cast<T*>(p.k_out) + dst[e], wk[e], sk[e]);
+            if (p.v_out) store_values(static_cast<T*>(p.v_out) + dst[e], wv[e], sv[e]);
         }
     }
 }
@@ -366,8 +378,8 @@ cudaError_t launch_kv8_append(int type, Kv8Append p, cudaStream_t st) {
 
 cudaError_t launch_kv8_read(int type, Kv8Read p, cudaStream_t st) {
     p.units = touched_pages(std::min(p.max_rows, p.n_tokens), p.c.page);
-    // about 16 KB of codes per CTA and tensor
-    p.heads_per_cta = std::max(1, std::min(p.c.n_kv, 16384 / (p.c.page * p.c.head_dim)));
+    // one round of loads per CTA
+    p.heads_per_cta = std::max(1, std::min(p.c.n_kv, kReadLoads * kThreads * 16 / (p.c.page * p.c.head_dim)));
     const int64_t ctas = (int64_t)p.c.n_seq * p.units * ceil_div(p.c.n_kv, p.heads_per_cta);
     if (type == TPTC_TYPE_F16) return read_t<__half>(p, ctas, st);
     if (type == TPTC_TYPE_BF16) return read_t<__nv_bfloat16>(p, ctas, st);
