@@ -122,6 +122,21 @@ def test_rows_without_a_distribution(cuda_device):
     assert run(x.to(cuda_device), K.F32, tokens[:1].to(cuda_device), 32)[2][0].tolist() == list(range(32))
 
 
+@pytest.mark.parametrize("rows", [1, 300])
+def test_many_nan_and_infinite_logits(cuda_device, rows):
+    """NaN, then +inf, then the rest, by lowest index -- also where they fill some warps' lists."""
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(rows, 60000, generator=g)
+    x[:, 5000:5040] = math.nan
+    x[:, 40000:40003] = math.inf
+    x[:, 59990:] = math.nan
+    ids = run(x.to(cuda_device), K.F32, torch.zeros(rows, dtype=torch.int32, device=cuda_device), 32)[2]
+    assert (ids == torch.arange(5000, 5032)).all()
+    x[:, 5020:5040] = 0.0
+    ids = run(x.to(cuda_device), K.F32, torch.zeros(rows, dtype=torch.int32, device=cuda_device), 32)[2]
+    assert (ids == torch.tensor(list(range(5000, 5020)) + list(range(59990, 60000)) + [40000, 40001])).all()
+
+
 def test_parts_and_graph_replay(cuda_device):
     """What is not wanted is left out; a captured call replays on new logits, in any number of CTAs per row."""
     dev = cuda_device

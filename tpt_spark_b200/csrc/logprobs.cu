@@ -10,11 +10,11 @@
 // value bits, then ~index): keys are unique and their order is the wanted one.  Each warp keeps
 // its n largest sorted, lane i the i-th, and looks at a chunk's elements again only when one of
 // the 16-element maxima (which the online maximum needs anyway) reaches a threshold: the larger of
-// the warp's own n-th, of the n-th largest of the first chunk's 32 group maxima, and of the smallest
-// over the warps of their ceil(n / warps)-th, which they publish without a barrier (each bounds the
+// the warp's own n-th, of the n-th largest of the first chunk's 32 group maxima, and of the r-th largest
+// over the warps of their k-th, k r >= n, which they publish without a barrier (each bounds the
 // row's n-th from below, whenever it is read).  About n ln(vocab / chunk) elements of a row are
 // ever inserted.  (A shared candidate list with a barrier per chunk took 341 us for 1500 bf16 rows of 128256,
-// this takes 95 us; both with n = 5.)
+// this takes 90 us; both with n = 5.)
 //
 // One CTA per row streams the logits: HBM bound, with the exponentials (16 per cycle and SM) close
 // behind for 16-bit logits.  With few rows a cluster of CTAs shares one row and joins through
@@ -78,8 +78,8 @@ struct Shared {
 // out[0 .. n) in order.  Keys that are not 0 are unique, and 0 stands for nothing.
 __device__ __forceinline__ void merge_lists(const unsigned long long (*list)[kMaxTop], int lists, int n,
                                             unsigned long long* out) {
-    const int w = threadIdx.x / kMaxTop, i = threadIdx.x % kMaxTop;
-    if (w >= lists || i >= n) return;
+    if ((int)threadIdx.x >= lists * n) return;  // (few keys: few warps)
+    const int w = threadIdx.x / n, i = threadIdx.x - w * n;
     const unsigned long long mine = list[w][i];
     int before[kWarps];  // of list o, how many come before mine: a binary search, all lists at once
 #pragma unroll
@@ -159,7 +159,9 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const __grid_constant__ LogprobParams p, int parts) {
     constexpr int VEC = 16 / sizeof(T), U = kVecs, S = kStages, E = U * VEC, CHUNK = kThreads * E;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-    extern __shared__ __align__(16) uint8_t ring[];  // [S][U][kThreads] vectors, filled by the thread that sums them
+    // [S][U][kThreads] vectors, filled by the thread that sums them.  (128-byte aligned: copies to other places
+    // took three times the shared-memory passes and twice the sectors from L2.)
+    extern __shared__ __align__(128) uint8_t ring[];
     __shared__ Shared s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / parts, part = blockIdx.x % parts, n = p.n_top;
@@ -208,6 +210,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const __
     State st = {-INFINITY, 0.f, 0.f};
     float c = 0.f, delta = 0.f, scale = 1.f;  // of st.m: m log2 e rounded, what was cut off, and 2^-delta
     unsigned long long mine = 0;               // lane i: the warp's i-th largest key
+    // warps publish their k_share-th; the r_share-th largest of those bounds the n-th of all
+    const int k_share = (n + 4) / 5, r_share = n > 0 ? (n + k_share - 1) / k_share : 1;
     float thr = -INFINITY;
     for (int chunk = c0; chunk < c1; chunk++) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
@@ -320,13 +324,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const __
                     }
                 }
                 if (last) thr = fmaxf(thr, unordered((uint32_t)(last >> 32)));
-                const unsigned long long share = __shfl_sync(0xffffffffu, mine, (n - 1) / kWarps);
-                if (lane == 0 && share) s.published[warp] = unordered((uint32_t)(share >> 32));
+                const unsigned long long share = __shfl_sync(0xffffffffu, mine, k_share - 1);
+                if (lane == 0 && share) {
+                    const float f = unordered((uint32_t)(share >> 32));
+                    s.published[warp] = f == f ? f : INFINITY;  // (NaN counts as largest)
+                }
             }
             if (found || chunk % 4 == 0) {
-                float shared = s.published[lane % kWarps];
+                const float v = s.published[lane % kWarps];
+                int rank = 0;
 #pragma unroll
-                for (int o = 1; o < kWarps; o <<= 1) shared = fminf(shared, __shfl_xor_sync(0xffffffffu, shared, o));
+                for (int o = 1; o < kWarps; o++) {
+                    const float u = __shfl_xor_sync(0xffffffffu, v, o);
+                    rank += u > v || (u == v && (lane ^ o) < lane);
+                }
+                const float shared = __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, rank == r_share - 1)) - 1);
                 thr = fmaxf(thr, shared);
             }
         }

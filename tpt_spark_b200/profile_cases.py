@@ -7,6 +7,9 @@ launches the kernel a few times through the library's public entry points and ex
     python -m tpt_spark_b200.profile_cases attn_prefill 4096     # causal prefill attention, T
     python -m tpt_spark_b200.profile_cases attn_decode 8192      # decode attention (C5 heads), position
     python -m tpt_spark_b200.profile_cases prefill 2048          # C5 batched prefill, prompt tokens
+    python -m tpt_spark_b200.profile_cases attn_packed 4096      # packed prompt attention, T tokens of one prompt
+    python -m tpt_spark_b200.profile_cases kv8_attn 8 32768      # decode attention over the paged 8-bit cache: n, length
+    python -m tpt_spark_b200.profile_cases logprobs 600 128256   # log probabilities, rows and vocabulary
 
 The launch counts are what the summaries under profiles/ select with ncu's -s / -c.
 """
@@ -141,8 +144,62 @@ def prefill(P: int) -> None:
     print("prefill ms", e.last_device_ms())
 
 
+def attn_packed(T: int) -> None:
+    """tptc_attn_packed three times: one bf16 prompt of T tokens, 32 heads / 8 kv heads, head_dim 128."""
+    import torch
+
+    from . import kernels
+
+    H, KV, hd = 32, 8, 128
+    q, k, v = (torch.randn(T, h, hd, device="cuda").bfloat16() for h in (H, KV, KV))
+    o, cu = torch.empty_like(q), torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        kernels.attn_packed(q, k, v, o, kernels.BF16, H * hd, KV * hd, KV * hd, cu, cu, 1, T, T, T, H, KV, hd)
+    torch.cuda.synchronize()
+    print("ok", float(o[0, 0, 0]))
+
+
+def kv8_attn(n: int, length: int) -> None:
+    """tptc_kv8_attn three times: n sequences of `length` positions in shuffled pages of 64, 32 query
+    heads over 8 kv heads of 128, bf16 queries."""
+    import torch
+
+    from . import kernels
+
+    H, KV, hd, page = 32, 8, 128, 64
+    per = -(-length // page)
+    pages = n * per
+    k, v = (torch.randint(-127, 128, (pages, KV, page, hd), dtype=torch.int8, device="cuda") for _ in "kv")
+    ks, vs = torch.full((2, pages, KV), 0.01, device="cuda").unbind(0)
+    table = torch.randperm(pages, device="cuda").int().view(n, per)
+    cache = kernels.Kv8Cache(k, v, ks, vs, table, None, pages, page, KV, hd, n, per)
+    q = torch.randn(n, H, hd, device="cuda").bfloat16()
+    out, lens = torch.empty_like(q), torch.full((n,), length, dtype=torch.int32, device="cuda")
+    work = torch.zeros(cache.attn_workspace_bytes(H), dtype=torch.uint8, device="cuda")
+    for _ in range(3):
+        cache.attn(q, H * hd, kernels.BF16, lens, H, out, work, work.numel())
+    torch.cuda.synchronize()
+    print("ok", float(out[0, 0, 0]))
+
+
+def logprobs(rows: int, vocab: int) -> None:
+    """tptc_logprobs three times: bf16 logits, the five largest of each row."""
+    import torch
+
+    from . import kernels
+
+    x = (2.5 * torch.randn(rows, vocab, device="cuda")).bfloat16()
+    tokens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    lp, ent = torch.empty(2, rows, device="cuda").unbind(0)
+    ids, top = torch.empty(rows, 5, dtype=torch.int32, device="cuda"), torch.empty(rows, 5, device="cuda")
+    for _ in range(3):
+        kernels.logprobs(x, kernels.BF16, rows, vocab, vocab, tokens, lp, ent, 5, ids, top)
+    torch.cuda.synchronize()
+    print("ok", float(lp[0]))
+
+
 CASES = {"gemv": gemv, "gemm": gemm, "gemm_q": gemm_q, "attn_prefill": attn_prefill, "attn_decode": attn_decode,
-         "prefill": prefill}
+         "prefill": prefill, "attn_packed": attn_packed, "kv8_attn": kv8_attn, "logprobs": logprobs}
 
 
 def main(argv=None) -> int:
