@@ -100,6 +100,21 @@ def test_calls_repeat_and_share_a_workspace(cuda_device):
     assert torch.equal(out, first)
 
 
+def test_one_workspace_for_batches_of_any_shape(cuda_device):
+    """A batch that grows and shrinks, other heads and widths: one workspace serves them all."""
+    shapes = [(3, 8, 2, 64, 900), (60, 32, 8, 128, 700), (2, 16, 1, 96, 3000), (60, 32, 8, 64, 300), (3, 8, 2, 64, 900)]
+    caches = []
+    for i, (n, H, n_kv, hd, most) in enumerate(shapes):
+        lens = [1 + (most * (7 * b + 3 * i + 1)) // 997 % most for b in range(n)]
+        c = make(lens, 16, n_kv, hd, 30 + i, cuda_device)
+        q = torch.randn(n, H, hd, device=cuda_device, generator=torch.Generator(cuda_device).manual_seed(i)).half()
+        caches.append((c, q, lens, run(c, q, K.F16, lens, cuda_device)))
+    work = torch.zeros(max(c.handle.attn_workspace_bytes(q.shape[1]) for c, q, _, _ in caches), dtype=torch.uint8,
+                       device=cuda_device)
+    for c, q, lens, want in caches + caches[::-1]:
+        assert torch.equal(run(c, q, K.F16, lens, cuda_device, work), want)
+
+
 @pytest.mark.parametrize("kind", [K.F16, K.BF16, K.F32])
 def test_pages_of_very_different_scales(cuda_device, kind):
     """A page of huge values that nearly no weight falls on, beside small ones that carry the output; a page of zeros."""

@@ -77,13 +77,13 @@ def test_rows_at_any_alignment(cuda_device, kind, offset):
     check(x, tokens, got, 9)
 
 
-@pytest.mark.parametrize("shape", ["ascending", "descending", "constant", "few values", "spread"])
+@pytest.mark.parametrize("shape", ["ascending", "descending", "constant", "few values", "spread", "huge"])
 @pytest.mark.parametrize("kind", [K.F32, K.BF16])
 def test_orders_and_ties(cuda_device, kind, shape):
     vocab = 70000
     i = torch.arange(vocab, dtype=torch.float64)
     x = {"ascending": i / 7000, "descending": -i / 7000, "constant": i * 0 + 1.5, "few values": (i * 7919 % 5),
-         "spread": (i * 7919 % vocab) / 3 - 20000}[shape]
+         "spread": (i * 7919 % vocab) / 3 - 20000, "huge": (i * 7919 % vocab) * 1e30}[shape]
     x = x.to(TYPES[kind])[None].repeat(2, 1)
     tokens = torch.tensor([0, vocab - 1], dtype=torch.int32)
     check(x, tokens, run(x.to(cuda_device), kind, tokens.to(cuda_device), 32), 32)

@@ -634,9 +634,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
 
 int grid_of(int sms) { return kCtasPerSm * sms; }
 int pairs_of(int n_heads, int n_kv) { return n_kv * ceil_div(n_heads / n_kv, kHeads); }
-size_t counter_bytes(const tptc_kv8& c, int n_heads) {
-    return ((size_t)c.n_seq * pairs_of(n_heads, c.n_kv) * sizeof(int) + 255) / 256 * 256;
-}
+// The records lie first, in room for the widest heads, and the counters behind them: a workspace that has served
+// one shape holds zero counters for every other that fits it.
+size_t record_bytes(int sms) { return (size_t)2 * grid_of(sms) * Lay<128>::kRecord * sizeof(float); }
 
 template <typename T, int HD>
 cudaError_t launch(const Params& p, int sms, cudaStream_t st) {
@@ -668,7 +668,7 @@ cudaError_t init_t() {
 }  // namespace
 
 size_t kv8_attn_workspace(const tptc_kv8& c, int n_heads, int sms) {
-    return counter_bytes(c, n_heads) + (size_t)2 * grid_of(sms) * (3 * kHeads + kHeads * c.head_dim) * sizeof(float);
+    return record_bytes(sms) + (size_t)c.n_seq * pairs_of(n_heads, c.n_kv) * sizeof(int);
 }
 
 cudaError_t launch_kv8_attn(int type, const Kv8Attn& a, int sms, cudaStream_t st) {
@@ -679,8 +679,8 @@ cudaError_t launch_kv8_attn(int type, const Kv8Attn& a, int sms, cudaStream_t st
     p.len = a.len;
     p.n_heads = a.n_heads;
     p.out = a.out;
-    p.counters = reinterpret_cast<int*>(a.workspace);
-    p.records = reinterpret_cast<float*>(a.workspace + counter_bytes(a.c, a.n_heads));
+    p.records = reinterpret_cast<float*>(a.workspace);
+    p.counters = reinterpret_cast<int*>(a.workspace + record_bytes(sms));
     p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)a.c.head_dim));
     if (type == TPTC_TYPE_F16) return launch_t<__half>(p, sms, st);
     if (type == TPTC_TYPE_BF16) return launch_t<__nv_bfloat16>(p, sms, st);

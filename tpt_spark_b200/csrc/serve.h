@@ -108,7 +108,7 @@ struct Kv8Attn {
     const int32_t* len;
     int n_heads;
     void* out;
-    uint8_t* workspace;  // kv8_attn_workspace() bytes; the counters at its head are zero between calls
+    uint8_t* workspace;  // kv8_attn_workspace() bytes; the counters at its end are zero between calls
 };
 size_t kv8_attn_workspace(const tptc_kv8& c, int n_heads, int sms);
 cudaError_t launch_kv8_attn(int type, const Kv8Attn& a, int sms, cudaStream_t st);
