@@ -103,6 +103,21 @@ def test_scores_that_climb_and_fall(cuda_device):
         check(got, reference(q, k, v, [n], [n]), v, K.F16)
 
 
+@pytest.mark.parametrize("n", [40, 300, 2500])
+def test_many_short_prompts_beside_long_ones(cuda_device, n):
+    """Tokens to decode and prompts of every length in one batch, in an order that is not sorted."""
+    hd, lq = 64, [1 + (i * 7919 % 5) * (i % 3 == 0) for i in range(n)]
+    for at, long in ((n // 3, 700), (n // 2, 300), (n - 1, 699), (7, 0)):
+        lq[at] = long
+    lk = [m + i % 4 * 5 for i, m in enumerate(lq)]
+    g = torch.Generator().manual_seed(n)
+    q, k, v = (torch.randn(m, h, hd, generator=g).half() for m, h in ((sum(lq), 2), (sum(lk), 1), (sum(lk), 1)))
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    got = run(q.to(cuda_device), k.to(cuda_device), v.to(cuda_device), K.F16, lq, lk, cuda_device, status=status)
+    assert int(status) == 0
+    check(got, reference(q, k, v, lq, lk), v, K.F16)
+
+
 def test_results_do_not_depend_on_the_batch(cuda_device):
     """A prompt alone, among others, and continued from a prefix: the same bits."""
     dev, hd = cuda_device, 128

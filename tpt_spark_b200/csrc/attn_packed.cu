@@ -17,7 +17,7 @@
 // Tried and slower: two threads per lane (519 us for 8192 tokens, 32 heads on 8, against 441), a quarter of the exponentials
 // as polynomials (483 against 462), P in the place of S with 128 keys per tile (448), turns of A
 // and B at the exponentials (470).
-// Measured there: 441 us = 1245 TFLOP/s.
+// Measured there: 440 us = 1250 TFLOP/s.
 //
 // Softmax: one thread per lane, base 2, with a reference maximum that moves (rescaling O in TMEM and
 // the f32 sum) only when a tile's maximum passes it by 8, so P stays below 2^8.
@@ -34,7 +34,7 @@ namespace tptc {
 namespace {
 
 constexpr int BM = 128;
-constexpr int kThreads = 384;  // warpgroup 0: copies (warp 0), products of A and B (1, 2); 1 and 2: their softmax
+constexpr int kThreads = 384;  // warpgroup 0: copies (warp 0), products of A and B (1, 2), items (3); 1 and 2: their softmax
 // Registers: 384 threads launch with 168 each; the softmax threads hold 128 scores and take what
 // warpgroup 0 gives back (128 x (72 + 2 x 216) = 384 x 168).
 constexpr int kRegsFew = 72, kRegsMany = 216;
@@ -58,7 +58,7 @@ struct Params {
     void* out;
     const int32_t *cu_q, *cu_k;
     int n_seq, n_q, n_k, max_q, n_heads, n_kv;
-    int tokens, pairs;  // tokens per tile; pairs of tiles of the longest sequence
+    int tokens;  // per tile
     float scale_log2;
     int32_t* status;
 };
@@ -208,28 +208,85 @@ __device__ __forceinline__ int taken_item(const uint4* response) {
     return got ? (int)x : -1;
 }
 
-struct Item {
-    int q0, k0;     // packed rows: the first token of tile A, the sequence's first key
-    int kvh;
-    int base, lk;   // tile A's first token sees base + 1 keys; keys of the sequence
-    int toks[2], nt[2], ntot;  // tokens of a tile, and the key tiles that its last token sees
-};
-// Every role decodes an item for itself, alike; false: nothing to do.
-template <int BN>
-__device__ __forceinline__ bool decode(const Params& p, int index, Item& w) {
-    // the pairs of tiles with the most keys first
-    const int per = p.n_kv * p.n_seq, pair = p.pairs - 1 - index / per, at = index % per, b = at / p.n_kv;
-    w.kvh = at % p.n_kv;
+// Pairs of tiles that sequence b has; 0 where there is nothing to do or its offsets are out of range.
+__device__ __forceinline__ int pairs_of(const Params& p, int b, bool report) {
     const int q_lo = p.cu_q[b], q_hi = p.cu_q[b + 1], k_lo = p.cu_k[b], k_hi = p.cu_k[b + 1];
-    if (q_lo == q_hi) return false;
+    if (q_lo == q_hi) return 0;
     if (q_lo < 0 || q_hi < q_lo || q_hi > p.n_q || q_hi - q_lo > p.max_q || k_lo < 0 || k_hi < k_lo || k_hi > p.n_k) {
-        if (pair == 0 && threadIdx.x == 0 && p.status) atomicExch(p.status, TPTC_ERR_ARG);
+        if (report && p.status) atomicExch(p.status, TPTC_ERR_ARG);
+        return 0;
+    }
+    return (q_hi - q_lo - 1) / (2 * p.tokens) + 1;
+}
+
+struct alignas(16) Item {
+    int q0, k0;     // packed rows: the first token of tile A, the sequence's first key
+    int base, lk;   // tile A's first token sees base + 1 keys; keys of the sequence
+    int toks[2], nt[2];  // tokens of a tile, and the key tiles that its last token sees
+    int kvh, ntot;  // ntot -1: no more items
+};
+
+// The list of items, walked by one warp: block index i is item i of the list (level, sequence, kv head), where the
+// level is the number of a pair of tiles in its sequence, from the highest down: those with the most keys come first,
+// and nothing is launched for pairs that a short sequence does not have.  (With n_seq x longest indices,
+// 63 prompts of one token beside one of 8192 took 836 us instead of 440.)
+constexpr int kSeqs = 2048;  // sequences whose counts are kept in shared memory
+struct List {
+    const int* counts;  // [kSeqs]
+    int lo, hi;         // levels that the same sequences have (`count` of them): hi - 1 down to lo
+    int64_t before;     // the first place of level hi - 1 (places: items of a kv head)
+    int count;
+    int level, b0, skipped;  // of the last item found: its level, block of 32 sequences, and sequences before those
+    __device__ __forceinline__ int pairs(const Params& p, int b) const {
+        return b < p.n_seq ? (b < kSeqs ? counts[b] : pairs_of(p, b, false)) : 0;
+    }
+    __device__ __forceinline__ void levels_below(const Params& p, int top) {  // hi = top
+        hi = top;
+        count = 0;
+        int next = 0;
+        for (int b = 0; b < p.n_seq; b += 32) {
+            const int n = pairs(p, b + (threadIdx.x & 31));
+            count += __popc(__ballot_sync(0xffffffffu, n >= hi));
+            next = max(next, n < hi ? n : 0);
+        }
+        lo = __reduce_max_sync(0xffffffffu, next);
+    }
+    // sequence of place k, and its level (places only ever ascend); false: behind the last
+    __device__ __forceinline__ bool find(const Params& p, int k, int& b) {
+        if (p.n_seq == 1) {  // (a level has one place)
+            b = 0;
+            level = hi - 1 - k;
+            return level >= 0;
+        }
+        while (hi > 0 && k - before >= (int64_t)(hi - lo) * count) {
+            before += (int64_t)(hi - lo) * count;
+            if (lo > 0) levels_below(p, lo);
+            else hi = 0;
+        }
+        if (hi == 0) return false;
+        const int at_k = (int)(k - before), down = at_k / count, r = at_k - down * count, lane = threadIdx.x & 31;
+        if (hi - 1 - down != level) level = hi - 1 - down, b0 = skipped = 0;
+        for (; b0 < p.n_seq; b0 += 32) {
+            const bool has = pairs(p, b0 + lane) > level;
+            const uint32_t m = __ballot_sync(0xffffffffu, has);
+            const uint32_t at = __ballot_sync(0xffffffffu, has && skipped + __popc(m & ((1u << lane) - 1)) == r);
+            if (at) {
+                b = b0 + __ffs(at) - 1;
+                return true;
+            }
+            skipped += __popc(m);
+        }
         return false;
     }
-    const int lq = q_hi - q_lo, lk = k_hi - k_lo, tok0 = pair * 2 * p.tokens;
-    if (tok0 >= lq) return false;
+};
+template <int BN>
+__device__ __forceinline__ Item item_of(const Params& p, int b, int pair, int kvh) {
+    const int q_lo = p.cu_q[b], lq = p.cu_q[b + 1] - q_lo, k_lo = p.cu_k[b], lk = p.cu_k[b + 1] - k_lo;
+    const int tok0 = pair * 2 * p.tokens;
+    Item w;
     w.q0 = q_lo + tok0;
     w.k0 = k_lo;
+    w.kvh = kvh;
     w.lk = lk;
     w.base = lk - lq + tok0;
 #pragma unroll
@@ -239,8 +296,10 @@ __device__ __forceinline__ bool decode(const Params& p, int index, Item& w) {
         w.nt[t] = w.toks[t] > 0 && sees > 0 ? (sees + BN - 1) / BN : 0;
     }
     w.ntot = max(w.nt[0], w.nt[1]);
-    return true;
+    return w;
 }
+
+constexpr int kLead = 4;  // key tiles of an item still to load when the next one is asked for
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -250,9 +309,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int S = L::kStages, KS = HD / 16, BN = L::BN;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t q_full, q_empty, full[S], empty[S], item_full[2], item_empty[2];
+    __shared__ uint64_t q_full, q_empty, full[S], empty[S], item_full[2], item_empty[2], wanted, taken;
     __shared__ uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2], drain[2];
-    __shared__ uint4 response[2];
+    __shared__ uint4 response;
+    __shared__ Item items[2];
+    __shared__ int counts[kSeqs];
     __shared__ uint32_t tmem_slot;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = p.n_heads / p.n_kv;
@@ -271,25 +332,35 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&pv_done[t], 1);
             mbar_init(&drain[t], 1);
             mbar_init(&item_full[t], 1);
-            mbar_init(&item_empty[t], 10);  // two product warps and eight softmax warps have read it
+            mbar_init(&item_empty[t], 11);  // copies, two product warps and eight softmax warps have read it
         }
+        mbar_init(&wanted, 1);
+        mbar_init(&taken, 1);
         fence_mbar_init();
     }
     if (warp == 1) tmem_alloc(&tmem_slot, kTmemCols);
+    int most = 0;  // pairs of tiles of a sequence (warp 3)
+    if (warp == 3) {
+        for (int b = lane; b < p.n_seq; b += 32) {
+            const int n = pairs_of(p, b, blockIdx.x == 0);
+            if (b < kSeqs) counts[b] = n;
+            most = max(most, n);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_phase(bar, parity, p.status); };
-    // the next item's index for a warp of the products or the softmax, which has had n of them (-1: no more)
-    auto next_item = [&](int n) {
-        const int s = (n - 1) & 1;
-        if (!wait(&item_full[s], ((n - 1) >> 1) & 1)) return -1;
-        const int index = taken_item(&response[s]);
-        fence_proxy_async_smem();  // read before the slot is written again
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&item_empty[s]);
-        return index;
+    // the n-th item of the CTA, for a lane (copies) or a warp; false: no more
+    auto get_item = [&](int n, Item& w, bool whole_warp) {
+        const int s = n & 1;
+        if (!wait(&item_full[s], (n >> 1) & 1)) return false;
+        w = items[s];
+        if (whole_warp) __syncwarp();
+        if (!whole_warp || lane == 0) mbar_arrive(&item_empty[s]);
+        return w.ntot >= 0;
     };
 
     if (warp < 4) {
@@ -297,44 +368,65 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp == 0 && lane == 0) {  // copies: Q_A, Q_B, then K_0, V_0, K_1, ... of each item
             int i0 = 0, nq = 0;        // loads into the ring and Q tiles so far
             bool ok = true;
-            int index = blockIdx.x;
-            for (int n = 1; ok; n++) {
-                Item w;
-                if (decode<BN>(p, index, w) && w.ntot > 0) {
-                    if (nq > 0) ok = mbar_wait_backoff(&q_empty, (nq - 1) & 1, p.status);
-                    if (!ok) break;
-                    nq++;
-                    mbar_expect_tx(&q_full, (w.toks[1] > 0 ? 2 : 1) * ((uint32_t)(p.tokens * G) * 128 * L::NC));
-                    for (int t = 0; t < 2; t++) {
-                        if (w.toks[t] == 0) continue;
+            Item w;
+            for (int n = 0; ok && get_item(n, w, false); n++) {
+                if (w.ntot <= kLead) mbar_arrive(&wanted);
+                if (w.ntot == 0) continue;
+                if (nq > 0) ok = mbar_wait_backoff(&q_empty, (nq - 1) & 1, p.status);
+                if (!ok) break;
+                nq++;
+                mbar_expect_tx(&q_full, (w.toks[1] > 0 ? 2 : 1) * ((uint32_t)(p.tokens * G) * 128 * L::NC));
+                for (int t = 0; t < 2; t++) {
+                    if (w.toks[t] == 0) continue;
 #pragma unroll
-                        for (int c = 0; c < L::NC; c++)
-                            tma_load_3d(smem + t * L::kQTile + c * BM * 128, &tq, c * 64, w.kvh * G, w.q0 + t * p.tokens, &q_full);
-                    }
-                    for (int k = 0; k < 2 * w.ntot; k++, i0++) {
-                        const int s = i0 % S;
-                        if (i0 >= S) ok = mbar_wait_backoff(&empty[s], ((i0 / S) - 1) & 1, p.status);
-                        if (!ok) break;
-                        mbar_expect_tx(&full[s], L::kTile);
-#pragma unroll
-                        for (int c = 0; c < L::NC; c++)
-                            tma_load_3d(smem + L::kKV + s * L::kTile + c * BN * 128, (k & 1) ? &tv : &tk, c * 64, w.kvh,
-                                        w.k0 + (k >> 1) * BN, &full[s]);
-                    }
-                    if (!ok) break;
+                    for (int c = 0; c < L::NC; c++)
+                        tma_load_3d(smem + t * L::kQTile + c * BM * 128, &tq, c * 64, w.kvh * G, w.q0 + t * p.tokens, &q_full);
                 }
-                const int s = (n - 1) & 1;
-                if (n > 2) ok = mbar_wait_backoff(&item_empty[s], ((n - 3) >> 1) & 1, p.status);
-                if (!ok) break;
-                request_item(&response[s], &item_full[s]);
-                ok = mbar_wait_backoff(&item_full[s], ((n - 1) >> 1) & 1, p.status);
-                if (!ok) break;
-                index = taken_item(&response[s]);
-                if (index < 0) break;
+                for (int k = 0; k < 2 * w.ntot; k++, i0++) {
+                    const int s = i0 % S;
+                    if (i0 >= S) ok = mbar_wait_backoff(&empty[s], ((i0 / S) - 1) & 1, p.status);
+                    if (!ok) break;
+                    mbar_expect_tx(&full[s], L::kTile);
+#pragma unroll
+                    for (int c = 0; c < L::NC; c++)
+                        tma_load_3d(smem + L::kKV + s * L::kTile + c * BN * 128, (k & 1) ? &tv : &tk, c * 64, w.kvh,
+                                    w.k0 + (k >> 1) * BN, &full[s]);
+                    if (w.ntot > kLead && k == 2 * (w.ntot - kLead) - 1) mbar_arrive(&wanted);
+                }
             }
             // the copies still in flight land before the CTA exits
             if (nq > 0) wait_phase(&q_full, (nq - 1) & 1, nullptr);
             for (int k = i0 > S ? i0 - S : 0; k < i0; k++) wait_phase(&full[k % S], (k / S) & 1, nullptr);
+        }
+        if (warp == 3) {  // items: the CTA's own, then those taken over when the copies of the last near their end
+            List list = {counts, 0, most, 0, 0, -1, 0, 0};  // (no level yet)
+            if (most > 0 && p.n_seq > 1) list.levels_below(p, most);
+            int index = blockIdx.x;
+            for (int n = 0, taken_n = 0;;) {
+                Item w;
+                w.ntot = -1;
+                int b = 0;
+                const bool some = index >= 0 && list.find(p, index / p.n_kv, b);
+                if (some) w = item_of<BN>(p, b, list.level, index % p.n_kv);
+                if (some || index < 0) {
+                    const int s = n & 1;
+                    if (n >= 2 && !wait(&item_empty[s], ((n >> 1) - 1) & 1)) break;
+                    if (lane == 0) {
+                        items[s] = w;
+                        mbar_arrive(&item_full[s]);
+                    }
+                    if (index < 0) break;
+                    if (!wait(&wanted, n & 1)) index = -1;
+                    n++;
+                }
+                if (index < 0) continue;
+                // (an index behind the list's end takes over the next at once, until none is left)
+                if (lane == 0) request_item(&response, &taken);
+                index = wait(&taken, taken_n & 1) ? taken_item(&response) : -1;
+                taken_n++;
+                fence_proxy_async_smem();  // read before the slot is written again
+                __syncwarp();
+            }
         }
         if (warp == 1 || warp == 2) {  // products of a tile: the whole warp waits, one elected lane issues
             const int t = warp - 1;
@@ -381,15 +473,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 return true;
             };
             bool ok = true;
-            int index = blockIdx.x;
-            Item w, next;
-            bool work = decode<BN>(p, index, w), next_work = false;
-            for (int n = 1; index >= 0; n++, work = next_work, w = next) {
-                if (!work || w.ntot == 0) {
-                    index = next_item(n);
-                    next_work = index >= 0 && decode<BN>(p, index, next);
-                    continue;
-                }
+            Item w;
+            for (int n = 0; ok && get_item(n, w, true); n++) {
+                if (w.ntot == 0) continue;
                 const int nt = t ? w.nt[1] : w.nt[0];
                 ok = wait(&q_full, nq & 1) && wait_full(i0);
                 if (!ok) break;
@@ -405,15 +491,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (!ok) break;
                         commit(&empty[ik % S]);
                         if (j + 2 == w.ntot) commit(&q_empty);
-                    } else {  // the loads are all issued: the next item is known soon
-                        index = next_item(n);
-                        next_work = index >= 0 && decode<BN>(p, index, next);
                     }
                     ok = wait_full(iv);
                     if (ok && j < nt) ok = issue_pv(iv, j == 0);
                     if (ok) commit(&empty[iv % S]);
                 }
-                if (!ok) break;
                 i0 += 2 * w.ntot;
             }
             // every product issued has completed before TMEM is freed
@@ -428,15 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t tS = tmem + t * BN + loff, tP = tmem + L::kP + t * (BN / 2) + loff, tO = tmem + L::kO + t * HD + loff;
         int i0 = 0, ns = 0;  // loads and score tiles so far
         bool ok = true;
-        int index = blockIdx.x;
-        Item w, next;
-        bool work = decode<BN>(p, index, w), next_work = false;
-        for (int n = 1; index >= 0; n++, work = next_work, w = next) {
-            if (!work) {
-                index = next_item(n);
-                next_work = index >= 0 && decode<BN>(p, index, next);
-                continue;
-            }
+        Item w;
+        for (int n = 0; get_item(n, w, true); n++) {
             const int nt = t ? w.nt[1] : w.nt[0], toks = t ? w.toks[1] : w.toks[0];
             const int tok = t * p.tokens + min(r / G, max(toks - 1, 0));  // spare lanes follow the last token
             const int sees = w.base + tok + 1, all_see = w.base + t * p.tokens + 1;  // keys of this lane, and of every lane
@@ -536,8 +611,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 l += sum[0].x + sum[0].y;
             }
             if (!ok) break;
-            index = next_item(n);
-            next_work = index >= 0 && decode<BN>(p, index, next);
             if (nt > 0) {
                 ok = wait(&pv_done[t], (ns - 1) & 1);
                 if (!ok) break;
@@ -586,9 +659,11 @@ cudaError_t launch(const AttnPacked& a, Params p, cudaStream_t st) {
     if (e == cudaSuccess && a.n_k > 0) e = make_tmap_heads(&tv, a.v, bf, HD, a.n_kv, a.n_k, a.v_stride, 1, Lay<HD>::BN);
     if (e != cudaSuccess) return e;
     if (a.n_k == 0) tk = tv = tq;  // no key: no copy is made
-    const int64_t pairs = ceil_div64(std::min(a.max_q, a.n_q), 2 * p.tokens), ctas = pairs * a.n_kv * a.n_seq;
+    // pairs of tiles: no sequence has more than the longest, and together they have at most one that is not full each
+    const int64_t pairs = std::min((int64_t)a.n_seq * ceil_div64(std::min(a.max_q, a.n_q), 2 * p.tokens),
+                                   (int64_t)a.n_q / (2 * p.tokens) + a.n_seq);
+    const int64_t ctas = pairs * a.n_kv;
     if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    p.pairs = (int)pairs;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kThreads);
