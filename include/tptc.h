@@ -344,8 +344,9 @@ TPTC_API int tptc_attn_decode_noalloc_status(void* stream, int* out_code);
  * of the sequences in the packed row arrays (d_cu[0] >= 0, d_cu[n_seq] <= the row count that
  * the call is given; rows outside are neither read nor written), and a host bound on the
  * longest sequence sizes the launch.  Indices that live on the device are checked there: a
- * sequence whose offsets, positions or length are out of range is left out, and a page id
- * outside the cache is not followed; either sets *status to TPTC_ERR_ARG. */
+ * sequence whose offsets, positions or length are out of range is left out (behind offsets that
+ * descend, later ones may be as well), and a page id outside the cache is not followed; either sets
+ * *status to TPTC_ERR_ARG. */
 
 /* A paged KV cache in 8 bits: page p holds `page` consecutive positions of one sequence, for
  * every kv head; code c of page p and head h stands for c * scale[p][h]. */
@@ -382,7 +383,7 @@ typedef struct {
  *   rope: NULL stores and copies without rotating.
  * One scale per (page, kv head): with a the largest magnitude of the new rows in the page,
  * s = max(s_old, a * (1/127)), where s_old counts only if earlier positions of the sequence lie in the
- * page; a new code is x / s rounded to nearest even, and where s grows the earlier codes c become c * s_old / s,
+ * page; a new code is x * (1 / s) rounded to nearest even, and where s grows the earlier codes c become c * s_old / s,
  * rounded.  A scale below the smallest normal float is 0.  A page that receives a value that is
  * not finite gets scale NaN, so whatever attends to it becomes NaN.  Rows of the page behind
  * the last new position keep their codes.  No two sequences of one call may append to the same page.

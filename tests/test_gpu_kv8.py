@@ -69,6 +69,9 @@ CASES = [
     (16, 1, 128, 64, K.F16, 16, False, [17, 0, 300], [129, 63, 1]),
     (2, 2, 128, 64, K.F16, 0, False, [1], [300]),  # no rotation
     (0, 3, 128, 16, K.BF16, 128, False, [0, 21], [40, 3]),  # no queries
+    # tokens to decode beside prompts that are far longer
+    (2, 1, 64, 16, K.F16, 64, True, [i % 37 for i in range(41)], [400 if i == 17 else i % 3 for i in range(41)]),
+    (4, 2, 128, 32, K.BF16, 128, False, [i % 70 for i in range(300)], [600 if i in (0, 299) else 1 for i in range(300)]),
 ]
 
 
@@ -219,6 +222,30 @@ def test_read(cuda_device, kind, hd, page, n_kv):
     only = torch.full_like(out[1], 9.0)
     cache.read(cu, torch.tensor(start, dtype=torch.int32, device=dev), total + 4, 128, kind, None, only)
     assert torch.equal(only, out[1]) and int(c.dev["status"]) == 0
+
+
+@pytest.mark.parametrize("bad", [None, 0, 150, 299])
+def test_read_of_very_different_lengths(cuda_device, bad):
+    """One long sequence among 300 short ones; then one of them with positions behind its table."""
+    dev, hd, page, n_kv = cuda_device, 64, 16, 2
+    n = [900 if i == 70 else i % 4 + (i in (0, 299)) for i in range(300)]
+    n[150] = 2
+    start = [(i * 13) % 50 for i in range(300)]
+    c = Cache([a + b for a, b in zip(start, n)], page, n_kv, hd, seed=17)
+    cache, total = c.to(dev), sum(n)
+    cu = torch.tensor([0] + n).cumsum(0)
+    begin = torch.tensor(start, dtype=torch.int32)
+    if bad is not None:
+        begin[bad] = c.max_pages * page - 1 + (n[bad] == 1)
+    out = torch.full((2, total + 4, n_kv, hd), 9.0, device=dev)
+    cache.read(cu.int().to(dev), begin.to(dev), total + 4, 900, K.F32, out[0], out[1])
+    torch.cuda.synchronize()
+    assert int(c.dev["status"]) == (0 if bad is None else -1)
+    want = [torch.cat(x).float() for x in zip(*(c.values(b, m, s) for b, (s, m) in enumerate(zip(start, n))))]
+    for got, w in zip(out.cpu(), want):
+        if bad is not None:
+            w[cu[bad]:cu[bad + 1]] = 9
+        assert torch.equal(got[:total], w) and (got[total:] == 9).all()
 
 
 BAD = {

@@ -24,28 +24,84 @@ __device__ __forceinline__ void flag(int32_t* status) {
     if (status) atomicExch(status, TPTC_ERR_ARG);
 }
 
-// Rows [r0, r1) of sequence b lie in page `p` of its table; false when there are none.
+// The rows of sequence b (from packed row lo, position begin): how many, or -1 where they are out of range.
+__device__ __forceinline__ int rows_of(const tptc_kv8& c, const int32_t* cu, const int32_t* start, int n_rows, int most,
+                                       int rope_rows, int b, int& lo, int& begin) {
+    lo = cu[b];
+    begin = start[b];
+    const int hi = cu[b + 1];
+    if (lo == hi) return 0;
+    const int64_t cap = c.max_pages * c.page, end = (int64_t)begin + hi - lo;
+    const bool in = lo >= 0 && hi > lo && hi <= n_rows && hi - lo <= most && begin >= 0 && end <= cap &&
+                    (rope_rows < 0 || end <= rope_rows);
+    return in ? hi - lo : -1;
+}
+
+// A CTA's work: the rows of sequence b that lie in one page (page u of those that it touches).
 struct Span {
     int first, n;   // packed row of the first, and how many
     int off;        // their first row in the page
     int pos;        // position of the first
     int64_t entry;  // of the page table
 };
-__device__ __forceinline__ bool page_span(const tptc_kv8& c, const int32_t* cu, const int32_t* start, int n_rows,
-                                          int most, int rope_rows, int b, int u, Span& s) {
-    const int lo = cu[b], hi = cu[b + 1], begin = start[b];
-    if (lo == hi) return false;
-    const int64_t cap = (int64_t)c.max_pages * c.page, end = (int64_t)begin + hi - lo;
-    if (lo < 0 || hi < lo || hi > n_rows || hi - lo > most || begin < 0 || end > cap || (rope_rows >= 0 && end > rope_rows)) {
-        if (u == 0 && threadIdx.x == 0) flag(c.status);
-        return false;
+// The k-th page that any sequence touches, in order, as (sequence, its page); -1 behind the last.  (A call: it is
+// over before the rows' registers are in use.)
+__device__ __noinline__ int2 counted_unit(const tptc_kv8& c, const int32_t* cu, const int32_t* start, int n_rows, int most,
+                                          int rope_rows, int k) {
+    __shared__ int s_sum[kThreads / 32], s_at[2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, shift = 31 - __clz(c.page);
+    int before = 0;
+    for (int b0 = 0; b0 < c.n_seq; b0 += kThreads) {
+        const int b = b0 + threadIdx.x;
+        int lo, begin;
+        const int n = b < c.n_seq ? rows_of(c, cu, start, n_rows, most, rope_rows, b, lo, begin) : 0;
+        if (n < 0 && blockIdx.x == 0) flag(c.status);
+        const int t = n > 0 ? ((begin + n - 1) >> shift) - (begin >> shift) + 1 : 0;
+        int incl = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) s_sum[warp] = incl;
+        __syncthreads();
+        int lead = before;
+        for (int w = 0; w < kThreads / 32; w++) {
+            if (w < warp) lead += s_sum[w];
+            before += s_sum[w];
+        }
+        lead += incl - t;
+        if (lead <= k && k < lead + t) s_at[0] = b, s_at[1] = k - lead;
+        __syncthreads();
+        if (k < before && blockIdx.x != 0) break;  // (the first CTA sees all, and reports)
     }
-    const int64_t p = begin / c.page + u, r0 = max((int64_t)begin, p * c.page), r1 = min(end, (p + 1) * c.page);
-    if (r0 >= r1) return false;
-    s.first = lo + (int)(r0 - begin);
-    s.n = (int)(r1 - r0);
-    s.off = (int)(r0 - p * c.page);
-    s.pos = (int)r0;
+    return k < before ? make_int2(s_at[0], s_at[1]) : make_int2(-1, 0);
+}
+
+// units > 0: unit k is page k % units of sequence k / units.  units 0: units are counted (a batch whose longest
+// sequence is far from the others: 63 sequences of one row beside one of 8192 took 289 us in the first form, 59 in
+// this one).
+__device__ __forceinline__ bool page_span(const tptc_kv8& c, const int32_t* cu, const int32_t* start, int n_rows,
+                                          int most, int rope_rows, int units, int k, Span& s) {
+    const int shift = 31 - __clz(c.page);
+    int b, u, lo, begin;
+    if (units > 0) {
+        b = k / units;
+        u = k - b * units;
+    } else {
+        const int2 at = counted_unit(c, cu, start, n_rows, most, rope_rows, k);
+        if (at.x < 0) return false;
+        b = at.x;
+        u = at.y;
+    }
+    const int n = rows_of(c, cu, start, n_rows, most, rope_rows, b, lo, begin);
+    if (n < 0 && u == 0 && threadIdx.x == 0) flag(c.status);
+    const int p = (begin >> shift) + u, r0 = max(begin, p << shift), r1 = min(begin + n, (p << shift) + c.page);
+    if (n <= 0 || p > (begin + n - 1) >> shift) return false;
+    s.first = lo - begin + r0;
+    s.n = r1 - r0;
+    s.off = r0 & (c.page - 1);
+    s.pos = r0;
     s.entry = (int64_t)b * c.max_pages + p;
     return true;
 }
@@ -160,9 +216,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : NR == 4 ? 3 : 4
     const int tid = threadIdx.x, lg = tid % GS, grp = tid / GS, c = 8 * lg;
     const bool lane_in = c < HD;
     const int roles = p.q_out ? 2 : 1, role = blockIdx.x % roles, rest = blockIdx.x / roles;
-    const int h = rest % p.c.n_kv, unit = rest / p.c.n_kv, u = unit % p.units, b = unit / p.units;
+    const int h = rest % p.c.n_kv;
     Span s;
-    if (!page_span(p.c, p.cu, p.start, p.n_tokens, p.max_new, p.rope.dim ? p.rope.rows : -1, b, u, s)) return;
+    if (!page_span(p.c, p.cu, p.start, p.n_tokens, p.max_new, p.rope.dim ? p.rope.rows : -1, p.units, rest / p.c.n_kv, s)) return;
 
     if (role == 1) {  // the queries of this head group at the same positions: up to B heads of a token at a time
         constexpr int B = 4;
@@ -291,15 +347,15 @@ __device__ __forceinline__ void store_values(T* dst, const uint4& w, float scale
 
 // One CTA per (sequence, page, group of kv heads): 16 codes per load, kReadLoads of K and of V in flight per
 // thread; a page's rows of one head are contiguous, so that loads and stores both run along head_dim.  HBM bound:
-// 28 us for 21k positions of 8 heads of 128 (130 MB, 4.6 TB/s; 5.8 TB/s for ten times that), 3.7 us for 300.
+// 27 us for 21k positions of 8 heads of 128 (130 MB, 4.8 TB/s; 5.8 TB/s for ten times that), 3.5 us for 300.
 constexpr int kReadLoads = 2;  // (and 5 CTAs per SM: 255 us for 240k positions, 298 with 4 loads and 3 CTAs)
-template <typename T, int HD>
+template <typename T, int HD, bool COUNTED>  // (both forms in one kernel: 29.4 us for 27.1)
 __global__ void __launch_bounds__(kThreads, 5) kv8_read_kernel(const __grid_constant__ Kv8Read p) {
     constexpr int CH = HD / 16;
     const int groups = (p.c.n_kv + p.heads_per_cta - 1) / p.heads_per_cta;
-    const int g = blockIdx.x % groups, unit = blockIdx.x / groups, u = unit % p.units, b = unit / p.units;
+    const int g = blockIdx.x % groups;
     Span s;
-    if (!page_span(p.c, p.cu, p.start, p.n_tokens, p.max_rows, -1, b, u, s)) return;
+    if (!page_span(p.c, p.cu, p.start, p.n_tokens, p.max_rows, -1, COUNTED ? 0 : max(p.units, 1), blockIdx.x / groups, s)) return;
     const int page_id = p.c.table[s.entry];
     if (!in_cache(p.c, page_id)) return;
     const int h0 = g * p.heads_per_cta, heads = min(p.heads_per_cta, p.c.n_kv - h0);
@@ -356,31 +412,43 @@ cudaError_t append_t(const Kv8Append& p, int64_t ctas, cudaStream_t st) {
     return append_hd<T, 128>(p, ctas, st);
 }
 
-template <typename T>
-cudaError_t read_t(const Kv8Read& p, int64_t ctas, cudaStream_t st) {
-    if (p.c.head_dim == 64) return launch(kv8_read_kernel<T, 64>, ctas, p, st);
-    if (p.c.head_dim == 96) return launch(kv8_read_kernel<T, 96>, ctas, p, st);
-    return launch(kv8_read_kernel<T, 128>, ctas, p, st);
+template <typename T, int HD>
+cudaError_t read_hd(const Kv8Read& p, int64_t ctas, cudaStream_t st) {
+    if (p.units > 0) return launch(kv8_read_kernel<T, HD, false>, ctas, p, st);
+    return launch(kv8_read_kernel<T, HD, true>, ctas, p, st);
 }
 
-// Pages that n consecutive positions can touch, wherever they begin.
-int touched_pages(int n, int page) { return (int)(((int64_t)n + page - 2) / page + 1); }
+template <typename T>
+cudaError_t read_t(const Kv8Read& p, int64_t ctas, cudaStream_t st) {
+    if (p.c.head_dim == 64) return read_hd<T, 64>(p, ctas, st);
+    if (p.c.head_dim == 96) return read_hd<T, 96>(p, ctas, st);
+    return read_hd<T, 128>(p, ctas, st);
+}
+
+// Units to launch: n consecutive positions touch at most (n + page - 2) / page + 1 pages wherever they begin, all
+// sequences together two each beside those that their rows fill.  A unit without rows costs 2 ns (one with rows
+// about 20), counting 3 to 18 % of a launch: units are counted where that launches less than half as many.
+int64_t units_of(int n_seq, int n_tokens, int most, int page, int* units) {
+    const int64_t each = ((int64_t)std::min(most, n_tokens) + page - 2) / page + 1;
+    const int64_t straight = n_seq * each, listed = n_tokens / page + (int64_t)2 * n_seq;
+    *units = straight <= 2 * listed ? (int)each : 0;
+    return *units ? straight : listed;
+}
 
 }  // namespace
 
 cudaError_t launch_kv8_append(int type, Kv8Append p, cudaStream_t st) {
-    p.units = touched_pages(std::min(p.max_new, p.n_tokens), p.c.page);
-    const int64_t ctas = (int64_t)p.c.n_seq * p.units * p.c.n_kv * (p.q_out ? 2 : 1);
+    const int64_t ctas = units_of(p.c.n_seq, p.n_tokens, p.max_new, p.c.page, &p.units) * p.c.n_kv * (p.q_out ? 2 : 1);
     if (type == TPTC_TYPE_F16) return append_t<__half>(p, ctas, st);
     if (type == TPTC_TYPE_BF16) return append_t<__nv_bfloat16>(p, ctas, st);
     return append_t<float>(p, ctas, st);
 }
 
 cudaError_t launch_kv8_read(int type, Kv8Read p, cudaStream_t st) {
-    p.units = touched_pages(std::min(p.max_rows, p.n_tokens), p.c.page);
     // one round of loads per CTA
     p.heads_per_cta = std::max(1, std::min(p.c.n_kv, kReadLoads * kThreads * 16 / (p.c.page * p.c.head_dim)));
-    const int64_t ctas = (int64_t)p.c.n_seq * p.units * ceil_div(p.c.n_kv, p.heads_per_cta);
+    const int64_t ctas =
+        units_of(p.c.n_seq, p.n_tokens, p.max_rows, p.c.page, &p.units) * ceil_div(p.c.n_kv, p.heads_per_cta);
     if (type == TPTC_TYPE_F16) return read_t<__half>(p, ctas, st);
     if (type == TPTC_TYPE_BF16) return read_t<__nv_bfloat16>(p, ctas, st);
     return read_t<float>(p, ctas, st);

@@ -87,7 +87,7 @@ struct Kv8Append {
     void *q_out, *k_out;
     const int32_t *cu, *start;
     int n_tokens, max_new;
-    int units;  // pages that a sequence can touch (filled by the launcher)
+    int units;  // pages that a sequence can touch, 0: units are counted on the device (filled by the launcher)
 };
 cudaError_t launch_kv8_append(int type, Kv8Append p, cudaStream_t st);
 
@@ -96,7 +96,7 @@ struct Kv8Read {
     const int32_t *cu, *start;
     int n_tokens, max_rows;
     void *k_out, *v_out;
-    int units, heads_per_cta;  // filled by the launcher
+    int units, heads_per_cta;  // units as above; filled by the launcher
 };
 cudaError_t launch_kv8_read(int type, Kv8Read p, cudaStream_t st);
 
