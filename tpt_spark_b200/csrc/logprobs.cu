@@ -14,7 +14,7 @@
 // over the warps of their k-th, k r >= n, which they publish without a barrier (each bounds the
 // row's n-th from below, whenever it is read).  About n ln(vocab / chunk) elements of a row are
 // ever inserted.  (A shared candidate list with a barrier per chunk took 341 us for 1500 bf16 rows of 128256,
-// this takes 90 us; both with n = 5.)
+// this takes 88 us; both with n = 5.)
 //
 // One CTA per row streams the logits: HBM bound, with the exponentials (16 per cycle and SM) close
 // behind for 16-bit logits.  With few rows a cluster of CTAs shares one row and joins through
@@ -174,29 +174,33 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const __
     const int chunks = (int)((end + CHUNK - 1) / CHUNK), inner0 = shift ? 1 : 0, inner1 = (int)(end / CHUNK);
     const int c0 = (int)((int64_t)chunks * part / parts), c1 = (int)((int64_t)chunks * (part + 1) / parts);
 
-    const uint4* vectors = reinterpret_cast<const uint4*>(x - shift) + tid;
+    constexpr uint32_t kSlot = U * kThreads * 16;  // bytes of a chunk
+    const uint4* next = reinterpret_cast<const uint4*>(x - shift) + tid + (int64_t)c0 * (U * kThreads);  // to be loaded
     const uint32_t slots = smem_u32(ring) + tid * 16;
+    uint32_t to_slot = 0, slot = 0;  // bytes into the ring: of the next load, of the chunk at hand
+    const int whole0 = inner0, whole1 = min(inner1, c1);
     auto copy = [&](uint32_t dst, const uint4* src) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     };
     auto load = [&](int chunk) {  // chunks behind the last are not read
-        const uint32_t dst = slots + (chunk - c0) % S * (U * kThreads * 16);
-        const uint4* src = vectors + (int64_t)chunk * (U * kThreads);
-        if (chunk >= inner0 && chunk < min(inner1, c1)) {
+        const uint32_t dst = slots + to_slot;
+        if (chunk >= whole0 && chunk < whole1) {
 #pragma unroll
-            for (int u = 0; u < U; u++) copy(dst + u * kThreads * 16, src + u * kThreads);
+            for (int u = 0; u < U; u++) copy(dst + u * kThreads * 16, next + u * kThreads);
         } else if (chunk < c1) {  // an end of the row
 #pragma unroll 1
             for (int u = 0; u < U; u++) {
                 const int64_t e0 = (int64_t)chunk * CHUNK + (u * kThreads + tid) * VEC - shift;
                 if (e0 >= 0 && e0 + VEC <= p.vocab) {
-                    copy(dst + u * kThreads * 16, src + u * kThreads);
+                    copy(dst + u * kThreads * 16, next + u * kThreads);
                     continue;
                 }
-                T* to = reinterpret_cast<T*>(ring + ((chunk - c0) % S * U + u) * (kThreads * 16) + tid * 16);
+                T* to = reinterpret_cast<T*>(ring + to_slot + (u * kThreads + tid) * 16);
                 for (int i = 0; i < VEC; i++) to[i] = e0 + i >= 0 && e0 + i < p.vocab ? x[e0 + i] : static_cast<T>(-INFINITY);
             }
         }
+        next += U * kThreads;
+        to_slot = to_slot == (S - 1) * kSlot ? 0 : to_slot + kSlot;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // place in the row of element i of the E elements of thread t in a chunk
@@ -215,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const __
     float thr = -INFINITY;
     for (int chunk = c0; chunk < c1; chunk++) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
-        const uint32_t src = slots + (chunk - c0) % S * (U * kThreads * 16);
+        const uint32_t src = slots + slot;
         float mx = -INFINITY;
         uint32_t r[U * 4];
 #pragma unroll
@@ -309,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const __
                     unsigned long long key = 0;
                     if (lane < E && e >= 0 && e < p.vocab) {
                         const float v = to_f32(*reinterpret_cast<const T*>(
-                            ring + ((chunk - c0) % S * U + lane / VEC) * (kThreads * 16) + t * 16 + lane % VEC * sizeof(T)));
+                            ring + slot + lane / VEC * (kThreads * 16) + t * 16 + lane % VEC * sizeof(T)));
                         if (!(v < thr)) key = ((unsigned long long)ordered(v) << 32) | (uint32_t)~(uint32_t)e;
                     }
                     uint32_t todo = __ballot_sync(0xffffffffu, key > last);
@@ -342,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) logprobs_kernel(const __
                 thr = fmaxf(thr, shared);
             }
         }
+        slot = slot == (S - 1) * kSlot ? 0 : slot + kSlot;
     }
 
     // the CTA's state and list
