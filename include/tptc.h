@@ -343,7 +343,8 @@ TPTC_API int tptc_attn_decode_noalloc_status(void* stream, int* out_code);
  * Ragged batches are described by device arrays: d_cu[n_seq + 1] are the ascending row offsets
  * of the sequences in the packed row arrays (d_cu[0] >= 0, d_cu[n_seq] <= the row count that
  * the call is given; rows outside are neither read nor written), and a host bound on the
- * longest sequence sizes the launch.  Indices that live on the device are checked there: a
+ * longest sequence sizes the launch.  A call without rows or sequences does nothing and takes NULL
+ * for their arrays.  Indices that live on the device are checked there: a
  * sequence whose offsets, positions or length are out of range is left out (behind offsets that
  * descend, later ones may be as well), and a page id outside the cache is not followed; either sets
  * *status to TPTC_ERR_ARG. */

@@ -117,6 +117,16 @@ def test_nothing_to_do_is_no_error():
     logprobs(rows=0)
 
 
+def test_empty_arrays_may_be_null():
+    append(n_tokens=0, d_q=None, d_k=0, d_v=0, d_q_out=None, d_k_out=None, n_heads=0)
+    append(n_tokens=0, d_q=None, d_k=0, d_v=0)
+    append(cache(n_seq=0, d_table=0), d_cu=0, d_start=0)
+    read(n_tokens=0, d_k_out=None, d_v_out=P)
+    attn(cache(n_seq=0, d_table=0), d_q=0, d_len=0, d_out=0, d_workspace=0)
+    packed(n_q=0, d_q=0, d_out=0)
+    logprobs(rows=0, d_logits=0, d_token=None, d_logprob=P, d_top_id=None)
+
+
 def logprobs(**kw):
     a = dict(d_logits=P, type_=K.F32, rows=2, vocab=100, row_stride=100, d_token=P, d_logprob=P, d_entropy=P, n_top=5, d_top_id=P,
              d_top_logprob=P)

@@ -601,7 +601,7 @@ TPTC_API int tptc_block_dots(const tptc_matrix* m, const float* d_x, int32_t* d_
 static bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
 static int kv8_args(const tptc_kv8* c, int type) {
-    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || !c->table)
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || (!c->table && c->n_seq != 0))
         return fail_code(nullptr, TPTC_ERR_ARG, "kv8: null cache pointer");
     if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128)
         return fail_code(nullptr, TPTC_ERR_UNSUPPORTED, "kv8: head_dim must be 64, 96 or 128");
@@ -630,13 +630,14 @@ TPTC_API int tptc_kv8_append(const tptc_kv8* cache, const tptc_rope* rope, int t
                              int n_tokens, int max_new, void* stream) {
     if (int rc = kv8_args(cache, type)) return rc;
     if (n_tokens < 0 || max_new < 0) return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: negative row count");
-    if (!d_k || !d_v || !d_cu || !d_start) return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: null pointer");
+    const bool nothing = n_tokens == 0 || max_new == 0 || cache->n_seq == 0;  // (needs no rows and no offsets)
+    if (!nothing && (!d_k || !d_v || !d_cu || !d_start)) return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: null pointer");
     const int hd = cache->head_dim;
     if (bad_rows(d_k, k_stride, (int64_t)cache->n_kv * hd, type) || bad_rows(d_v, v_stride, (int64_t)cache->n_kv * hd, type) ||
         misaligned(d_k_out, 16))
         return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: k and v rows must be 16-byte aligned and not overlap");
     if (d_q_out) {
-        if (!d_q || n_heads <= 0 || n_heads % cache->n_kv)
+        if ((!d_q && !nothing) || n_heads <= 0 || n_heads % cache->n_kv)
             return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: n_heads must be a positive multiple of n_kv");
         if (bad_rows(d_q, q_stride, (int64_t)n_heads * hd, type) || misaligned(d_q_out, 16))
             return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: q rows must be 16-byte aligned and not overlap");
@@ -645,7 +646,7 @@ TPTC_API int tptc_kv8_append(const tptc_kv8* cache, const tptc_rope* rope, int t
                  rope->dim <= 0 || rope->dim % 16 || rope->dim > hd))
         return fail_code(nullptr, TPTC_ERR_ARG,
                          "kv8_append: rope tables must be 16-byte aligned, dim a multiple of 16 up to head_dim");
-    if (n_tokens == 0 || max_new == 0 || cache->n_seq == 0) return TPTC_OK;
+    if (nothing) return TPTC_OK;
     tptc::Kv8Append p = {};
     p.c = *cache;
     if (rope) p.rope = *rope;
@@ -670,9 +671,10 @@ TPTC_API int tptc_kv8_read(const tptc_kv8* cache, int type, const int32_t* d_cu,
                            int max_rows, void* d_k_out, void* d_v_out, void* stream) {
     if (int rc = kv8_args(cache, type)) return rc;
     if (n_tokens < 0 || max_rows < 0) return fail_code(nullptr, TPTC_ERR_ARG, "kv8_read: negative row count");
-    if (!d_cu || !d_start || misaligned(d_k_out, 16) || misaligned(d_v_out, 16))
+    const bool nothing = n_tokens == 0 || max_rows == 0 || cache->n_seq == 0 || (!d_k_out && !d_v_out);
+    if ((!nothing && (!d_cu || !d_start)) || misaligned(d_k_out, 16) || misaligned(d_v_out, 16))
         return fail_code(nullptr, TPTC_ERR_ARG, "kv8_read: null offsets or misaligned output");
-    if (n_tokens == 0 || max_rows == 0 || cache->n_seq == 0 || (!d_k_out && !d_v_out)) return TPTC_OK;
+    if (nothing) return TPTC_OK;
     tptc::Kv8Read p = {};
     p.c = *cache;
     p.cu = d_cu;
@@ -704,7 +706,8 @@ TPTC_API int64_t tptc_kv8_attn_workspace_bytes(const tptc_kv8* cache, int n_head
 TPTC_API int tptc_kv8_attn(const tptc_kv8* cache, int type, const void* d_q, int64_t q_stride, const int32_t* d_len,
                            int n_heads, void* d_out, void* d_workspace, int64_t workspace_bytes, void* stream) {
     if (int rc = kv8_attn_args(cache, type, n_heads)) return rc;
-    if (!d_q || !d_len || !d_out || !d_workspace) return fail_code(nullptr, TPTC_ERR_ARG, "kv8_attn: null pointer");
+    if (cache->n_seq > 0 && (!d_q || !d_len || !d_out || !d_workspace))
+        return fail_code(nullptr, TPTC_ERR_ARG, "kv8_attn: null pointer");
     if (bad_rows(d_q, q_stride, (int64_t)n_heads * cache->head_dim, type) || misaligned(d_out, 16) ||
         misaligned(d_workspace, 16))
         return fail_code(nullptr, TPTC_ERR_ARG, "kv8_attn: q rows, out and workspace must be 16-byte aligned");
@@ -736,7 +739,8 @@ TPTC_API int tptc_attn_packed(int type, const void* d_q, int64_t q_stride, const
         return fail_code(nullptr, TPTC_ERR_UNSUPPORTED, "attn_packed: type must be TPTC_TYPE_F16 or _BF16");
     if (head_dim != 64 && head_dim != 96 && head_dim != 128)
         return fail_code(nullptr, TPTC_ERR_UNSUPPORTED, "attn_packed: head_dim must be 64, 96 or 128");
-    if (!d_q || !d_k || !d_v || !d_out || !d_cu_q || !d_cu_k)
+    const bool nothing = n_seq == 0 || n_q == 0 || max_q == 0;  // (needs no pointer; without keys, none to them)
+    if (!nothing && (!d_q || !d_out || !d_cu_q || !d_cu_k || (n_k > 0 && (!d_k || !d_v))))
         return fail_code(nullptr, TPTC_ERR_ARG, "attn_packed: null pointer");
     if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv)
         return fail_code(nullptr, TPTC_ERR_ARG, "attn_packed: n_heads must be a positive multiple of n_kv");
@@ -747,7 +751,7 @@ TPTC_API int tptc_attn_packed(int type, const void* d_q, int64_t q_stride, const
     if (bad_rows(d_q, q_stride, (int64_t)n_heads * head_dim, type) || bad_rows(d_k, k_stride, (int64_t)n_kv * head_dim, type) ||
         bad_rows(d_v, v_stride, (int64_t)n_kv * head_dim, type) || misaligned(d_out, 32))
         return fail_code(nullptr, TPTC_ERR_ARG, "attn_packed: rows must be 16-byte aligned (out: 32) and not overlap");
-    if (n_seq == 0 || n_q == 0 || max_q == 0) return TPTC_OK;
+    if (nothing) return TPTC_OK;
     int dev = 0, sms = 0;
     if (int rc = ensure_kernels(&dev, &sms)) return rc;
     tptc::AttnPacked p = {};
@@ -777,10 +781,10 @@ TPTC_API int tptc_logprobs(int type, const void* d_logits, int rows, int vocab, 
                            float* d_top_logprob, void* stream) {
     if (type != TPTC_TYPE_F32 && type != TPTC_TYPE_F16 && type != TPTC_TYPE_BF16)
         return fail_code(nullptr, TPTC_ERR_UNSUPPORTED, "logprobs: type must be TPTC_TYPE_F32, _F16 or _BF16");
-    if (!d_logits || rows < 0 || vocab <= 0 || row_stride < vocab || misaligned(d_logits, type == TPTC_TYPE_F32 ? 4 : 2))
+    if ((!d_logits && rows != 0) || rows < 0 || vocab <= 0 || row_stride < vocab || misaligned(d_logits, type == TPTC_TYPE_F32 ? 4 : 2))
         return fail_code(nullptr, TPTC_ERR_ARG, "logprobs: bad logits");
-    if (!d_token != !d_logprob) return fail_code(nullptr, TPTC_ERR_ARG, "logprobs: d_token and d_logprob go together");
-    if (n_top < 0 || n_top > tptc::kMaxTop || n_top > vocab || (n_top > 0 && (!d_top_id || !d_top_logprob)))
+    if (rows != 0 && !d_token != !d_logprob) return fail_code(nullptr, TPTC_ERR_ARG, "logprobs: d_token and d_logprob go together");
+    if (n_top < 0 || n_top > tptc::kMaxTop || n_top > vocab || (rows > 0 && n_top > 0 && (!d_top_id || !d_top_logprob)))
         return fail_code(nullptr, TPTC_ERR_ARG, "logprobs: n_top must be 0 .. min(32, vocab), with both outputs");
     if (rows == 0) return TPTC_OK;
     int dev = 0, sms = 0;
