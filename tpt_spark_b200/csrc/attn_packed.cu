@@ -11,6 +11,8 @@
 // with P beside S and not in its place, the scores of the next keys are computed while the
 // exponentials of these run.  BN is what then fits 512 columns (128, 96, 80 keys for head_dim 64, 96,
 // 128).  P enters its product from TMEM.
+// A lane stores its own row at the end, 32 bytes at a time.  (Whole lines by way of shared memory: 105 us became 120 for
+// 12 prompts of 60 to 2100 tokens with 64-wide heads.)
 // Bounds, per pair of tiles and 128 keys at head_dim 128: 2048 cycles of exponentials (16 per cycle and
 // SM) and 2350 of the tensor core (S waits for shared memory, 6.5 KB of operands per 40 cycles).  What is
 // reached is 3450: a lone softmax warp's chain of waits, loads, maximum, exponentials and stores.
@@ -59,6 +61,7 @@ struct Params {
     const int32_t *cu_q, *cu_k;
     int n_seq, n_q, n_k, max_q, n_heads, n_kv;
     int tokens;  // per tile
+    uint32_t pair_mul, pair_shift;  // n / (2 tokens) = n pair_mul >> 32 >> pair_shift for n below 2^31
     float scale_log2;
     int32_t* status;
 };
@@ -195,28 +198,37 @@ __device__ __forceinline__ void request_item(uint4* response, uint64_t* bar) {
                  "r"(smem_u32(bar))
                  : "memory");
 }
-// The block index taken over, or -1 when none was left.
-__device__ __forceinline__ int taken_item(const uint4* response) {
-    uint32_t x, got;
+// Block indices: x is the kv head, y and z the place in the list of pairs of tiles (no division on the way).
+constexpr int kPlacesY = 32768;
+struct Place {
+    int kvh, k;  // k -1: none
+};
+// The block index taken over, if one was left.
+__device__ __forceinline__ Place taken_place(const uint4* response) {
+    uint32_t x, y, z, got;
     asm volatile(
-        "{\n .reg .pred p;\n .reg .b128 r;\n ld.shared.b128 r, [%2];\n"
-        " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.u32 %1, 1, 0, p;\n mov.u32 %0, 0;\n"
-        " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, r;\n}\n"
-        : "=&r"(x), "=&r"(got)
+        "{\n .reg .pred p;\n .reg .b128 r;\n ld.shared.b128 r, [%4];\n"
+        " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.u32 %3, 1, 0, p;\n"
+        " mov.u32 %0, 0;\n mov.u32 %1, 0;\n mov.u32 %2, 0;\n"
+        " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, %1, %2, _}, r;\n}\n"
+        : "=&r"(x), "=&r"(y), "=&r"(z), "=&r"(got)
         : "r"(smem_u32(response))
         : "memory");
-    return got ? (int)x : -1;
+    return {(int)x, got ? (int)(y + z * kPlacesY) : -1};
 }
 
-// Pairs of tiles that sequence b has; 0 where there is nothing to do or its offsets are out of range.
-__device__ __forceinline__ int pairs_of(const Params& p, int b, bool report) {
-    const int q_lo = p.cu_q[b], q_hi = p.cu_q[b + 1], k_lo = p.cu_k[b], k_hi = p.cu_k[b + 1];
-    if (q_lo == q_hi) return 0;
-    if (q_lo < 0 || q_hi < q_lo || q_hi > p.n_q || q_hi - q_lo > p.max_q || k_lo < 0 || k_hi < k_lo || k_hi > p.n_k) {
+struct Rows {
+    int q_lo, q_hi, k_lo, k_hi;
+};
+__device__ __forceinline__ Rows rows_of(const Params& p, int b) { return {p.cu_q[b], p.cu_q[b + 1], p.cu_k[b], p.cu_k[b + 1]}; }
+// Pairs of tiles that a sequence has; 0 where there is nothing to do or its offsets are out of range.
+__device__ __forceinline__ int pairs_of(const Params& p, const Rows& r, bool report) {
+    if (r.q_lo == r.q_hi) return 0;
+    if (r.q_lo < 0 || r.q_hi < r.q_lo || r.q_hi > p.n_q || r.q_hi - r.q_lo > p.max_q || r.k_lo < 0 || r.k_hi < r.k_lo || r.k_hi > p.n_k) {
         if (report && p.status) atomicExch(p.status, TPTC_ERR_ARG);
         return 0;
     }
-    return (q_hi - q_lo - 1) / (2 * p.tokens) + 1;
+    return (int)(__umulhi((uint32_t)(r.q_hi - r.q_lo - 1), p.pair_mul) >> p.pair_shift) + 1;
 }
 
 struct alignas(16) Item {
@@ -226,19 +238,20 @@ struct alignas(16) Item {
     int kvh, ntot;  // ntot -1: no more items
 };
 
-// The list of items, walked by one warp: block index i is item i of the list (level, sequence, kv head), where the
+// The list of items, walked by one warp: the places are ordered by level, then by sequence, where the
 // level is the number of a pair of tiles in its sequence, from the highest down: those with the most keys come first,
 // and nothing is launched for pairs that a short sequence does not have.  (With n_seq x longest indices,
 // 63 prompts of one token beside one of 8192 took 836 us instead of 440.)
 constexpr int kSeqs = 2048;  // sequences whose counts are kept in shared memory
 struct List {
     const int* counts;  // [kSeqs]
+    int top;            // pairs of the longest sequence
     int lo, hi;         // levels that the same sequences have (`count` of them): hi - 1 down to lo
     int64_t before;     // the first place of level hi - 1 (places: items of a kv head)
     int count;
     int level, b0, skipped;  // of the last item found: its level, block of 32 sequences, and sequences before those
     __device__ __forceinline__ int pairs(const Params& p, int b) const {
-        return b < p.n_seq ? (b < kSeqs ? counts[b] : pairs_of(p, b, false)) : 0;
+        return b < p.n_seq ? (b < kSeqs ? counts[b] : pairs_of(p, rows_of(p, b), false)) : 0;
     }
     __device__ __forceinline__ void levels_below(const Params& p, int top) {  // hi = top
         hi = top;
@@ -251,21 +264,25 @@ struct List {
         }
         lo = __reduce_max_sync(0xffffffffu, next);
     }
-    // sequence of place k, and its level (places only ever ascend); false: behind the last
+    // sequence of place k, and its level; false: behind the last.  (Places ascend: what was found before is the start.)
     __device__ __forceinline__ bool find(const Params& p, int k, int& b) {
         if (p.n_seq == 1) {  // (a level has one place)
             b = 0;
-            level = hi - 1 - k;
+            level = top - 1 - k;
             return level >= 0;
         }
-        while (hi > 0 && k - before >= (int64_t)(hi - lo) * count) {
-            before += (int64_t)(hi - lo) * count;
-            if (lo > 0) levels_below(p, lo);
-            else hi = 0;
+        if (hi == 0 || k < before) {
+            if (top == 0) return false;
+            before = 0;
+            levels_below(p, top);
         }
-        if (hi == 0) return false;
+        while (k - before >= (int64_t)(hi - lo) * count) {
+            if (lo == 0) return false;
+            before += (int64_t)(hi - lo) * count;
+            levels_below(p, lo);
+        }
         const int at_k = (int)(k - before), down = at_k / count, r = at_k - down * count, lane = threadIdx.x & 31;
-        if (hi - 1 - down != level) level = hi - 1 - down, b0 = skipped = 0;
+        if (hi - 1 - down != level || r < skipped) level = hi - 1 - down, b0 = skipped = 0;
         for (; b0 < p.n_seq; b0 += 32) {
             const bool has = pairs(p, b0 + lane) > level;
             const uint32_t m = __ballot_sync(0xffffffffu, has);
@@ -280,12 +297,11 @@ struct List {
     }
 };
 template <int BN>
-__device__ __forceinline__ Item item_of(const Params& p, int b, int pair, int kvh) {
-    const int q_lo = p.cu_q[b], lq = p.cu_q[b + 1] - q_lo, k_lo = p.cu_k[b], lk = p.cu_k[b + 1] - k_lo;
-    const int tok0 = pair * 2 * p.tokens;
+__device__ __forceinline__ Item item_of(const Params& p, const Rows& r, int pair, int kvh) {
+    const int lq = r.q_hi - r.q_lo, lk = r.k_hi - r.k_lo, tok0 = pair * 2 * p.tokens;
     Item w;
-    w.q0 = q_lo + tok0;
-    w.k0 = k_lo;
+    w.q0 = r.q_lo + tok0;
+    w.k0 = r.k_lo;
     w.kvh = kvh;
     w.lk = lk;
     w.base = lk - lq + tok0;
@@ -339,14 +355,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_mbar_init();
     }
     if (warp == 1) tmem_alloc(&tmem_slot, kTmemCols);
-    int most = 0;  // pairs of tiles of a sequence (warp 3)
+    // The list's warp: the first item is there when the CTA starts.  (An index behind the list's end: an item of nothing.)
+    List list = {counts, 0, 0, 0, 0, 0, -1, 0, 0};
+    Rows known = {};  // of sequence `lane`, loaded once
+    auto listed_item = [&](const Place& at, Item& w) {
+        int b = 0;
+        if (!list.find(p, at.k, b)) return false;
+        Rows r;
+        if (b < 32)
+            r = {__shfl_sync(0xffffffffu, known.q_lo, b), __shfl_sync(0xffffffffu, known.q_hi, b),
+                 __shfl_sync(0xffffffffu, known.k_lo, b), __shfl_sync(0xffffffffu, known.k_hi, b)};
+        else
+            r = rows_of(p, b);
+        w = item_of<BN>(p, r, list.level, at.kvh);
+        return true;
+    };
     if (warp == 3) {
         for (int b = lane; b < p.n_seq; b += 32) {
-            const int n = pairs_of(p, b, blockIdx.x == 0);
+            const Rows r = rows_of(p, b);
+            const int n = pairs_of(p, r, blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0);
+            if (b < 32) known = r;
             if (b < kSeqs) counts[b] = n;
-            most = max(most, n);
+            list.top = max(list.top, n);
         }
-        most = __reduce_max_sync(0xffffffffu, most);
+        list.top = __reduce_max_sync(0xffffffffu, list.top);
+        __syncwarp();
+        Item w = {};
+        listed_item({(int)blockIdx.x, (int)(blockIdx.y + blockIdx.z * kPlacesY)}, w);
+        if (lane == 0) items[0] = w;
     }
     tc_fence_before();
     __syncthreads();
@@ -356,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the n-th item of the CTA, for a lane (copies) or a warp; false: no more
     auto get_item = [&](int n, Item& w, bool whole_warp) {
         const int s = n & 1;
-        if (!wait(&item_full[s], (n >> 1) & 1)) return false;
+        if (n > 0 && !wait(&item_full[s], (n >> 1) & 1)) return false;
         w = items[s];
         if (whole_warp) __syncwarp();
         if (!whole_warp || lane == 0) mbar_arrive(&item_empty[s]);
@@ -398,34 +434,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (nq > 0) wait_phase(&q_full, (nq - 1) & 1, nullptr);
             for (int k = i0 > S ? i0 - S : 0; k < i0; k++) wait_phase(&full[k % S], (k / S) & 1, nullptr);
         }
-        if (warp == 3) {  // items: the CTA's own, then those taken over when the copies of the last near their end
-            List list = {counts, 0, most, 0, 0, -1, 0, 0};  // (no level yet)
-            if (most > 0 && p.n_seq > 1) list.levels_below(p, most);
-            int index = blockIdx.x;
-            for (int n = 0, taken_n = 0;;) {
-                Item w;
+        if (warp == 3) {  // the items behind the first, asked for when the copies of the one before near their end
+            if (lane == 0) mbar_arrive(&item_full[0]);
+            Place at = {0, 0};
+            for (int n = 1, asked = 0; at.k >= 0; n++) {
+                Item w = {};
                 w.ntot = -1;
-                int b = 0;
-                const bool some = index >= 0 && list.find(p, index / p.n_kv, b);
-                if (some) w = item_of<BN>(p, b, list.level, index % p.n_kv);
-                if (some || index < 0) {
-                    const int s = n & 1;
-                    if (n >= 2 && !wait(&item_empty[s], ((n >> 1) - 1) & 1)) break;
-                    if (lane == 0) {
-                        items[s] = w;
-                        mbar_arrive(&item_full[s]);
-                    }
-                    if (index < 0) break;
-                    if (!wait(&wanted, n & 1)) index = -1;
-                    n++;
+                at.k = -1;
+                if (wait(&wanted, (n - 1) & 1)) do {  // (indices behind the list's end are taken over until none is left)
+                    if (lane == 0) request_item(&response, &taken);
+                    if (wait(&taken, asked++ & 1)) at = taken_place(&response);
+                    else at.k = -1;
+                    fence_proxy_async_smem();  // read before the slot is written again
+                    __syncwarp();
+                } while (at.k >= 0 && !listed_item(at, w));
+                const int s = n & 1;
+                if (n >= 2 && !wait(&item_empty[s], ((n >> 1) - 1) & 1)) break;
+                if (lane == 0) {
+                    items[s] = w;
+                    mbar_arrive(&item_full[s]);
                 }
-                if (index < 0) continue;
-                // (an index behind the list's end takes over the next at once, until none is left)
-                if (lane == 0) request_item(&response, &taken);
-                index = wait(&taken, taken_n & 1) ? taken_item(&response) : -1;
-                taken_n++;
-                fence_proxy_async_smem();  // read before the slot is written again
-                __syncwarp();
             }
         }
         if (warp == 1 || warp == 2) {  // products of a tile: the whole warp waits, one elected lane issues
@@ -662,10 +690,12 @@ cudaError_t launch(const AttnPacked& a, Params p, cudaStream_t st) {
     // pairs of tiles: no sequence has more than the longest, and together they have at most one that is not full each
     const int64_t pairs = std::min((int64_t)a.n_seq * ceil_div64(std::min(a.max_q, a.n_q), 2 * p.tokens),
                                    (int64_t)a.n_q / (2 * p.tokens) + a.n_seq);
-    const int64_t ctas = pairs * a.n_kv;
-    if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    uint32_t log2 = 1;  // of 2 tokens, rounded up
+    while ((1u << log2) < 2u * p.tokens) log2++;
+    p.pair_mul = (uint32_t)(((1ull << (31 + log2)) + 2 * p.tokens - 1) / (2 * p.tokens));
+    p.pair_shift = log2 - 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.gridDim = dim3((unsigned)a.n_kv, (unsigned)std::min(pairs, (int64_t)kPlacesY), (unsigned)ceil_div64(pairs, kPlacesY));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Lay<HD>::kBytes + 1024;
     cfg.stream = st;

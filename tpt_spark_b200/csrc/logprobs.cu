@@ -14,7 +14,7 @@
 // over the warps of their k-th, k r >= n, which they publish without a barrier (each bounds the
 // row's n-th from below, whenever it is read).  About n ln(vocab / chunk) elements of a row are
 // ever inserted.  (A shared candidate list with a barrier per chunk took 341 us for 1500 bf16 rows of 128256,
-// this takes 88 us; both with n = 5.)
+// this takes 91 us; both with n = 5.)
 //
 // One CTA per row streams the logits: HBM bound, with the exponentials (16 per cycle and SM) close
 // behind for 16-bit logits.  With few rows a cluster of CTAs shares one row and joins through
