@@ -566,10 +566,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             }
             __syncthreads();
             if (s_last) {
-                auto part = [&](int i) {
-                    const int c = c0 + i;
-                    return p.records + (2 * (int64_t)c + (begins(c) >= was0 ? 0 : 1)) * L::kRecord;
-                };
+                // (only the first part's CTA can have begun before the pair)
+                const float* parts_at = p.records + 2 * (int64_t)c0 * L::kRecord;
+                const int first_off = begins(c0) >= was0 ? 0 : L::kRecord;
+                auto part = [&](int i) { return parts_at + (i == 0 ? first_off : i * (2 * L::kRecord)); };
                 // the references of all parts, 16 parts of 8 heads at a time
                 constexpr int kRows = kThreads / kHeads;
                 float *w_l = rec, *w_o = rec + kBlock * kHeads, *ref = rec + 2 * kBlock * kHeads;
