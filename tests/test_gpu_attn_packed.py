@@ -118,6 +118,17 @@ def test_many_short_prompts_beside_long_ones(cuda_device, n):
     check(got, reference(q, k, v, lq, lk), v, K.F16)
 
 
+def test_as_many_sequences_as_a_grid_has_rows(cuda_device):
+    """70000 tokens that see one key each: the output is that key's value."""
+    n, hd, dev = 70000, 64, cuda_device
+    q, k, v = (torch.randn(n, h, hd, device=dev).bfloat16() for h in (2, 1, 1))
+    cu, out = torch.arange(n + 1, dtype=torch.int32, device=dev), torch.zeros_like(q)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    K.attn_packed(q, k, v, out, K.BF16, 2 * hd, hd, hd, cu, cu, n, n, n, 1, 2, 1, hd, status)
+    torch.cuda.synchronize()
+    assert int(status) == 0 and torch.equal(out, v.expand(-1, 2, -1))
+
+
 def test_results_do_not_depend_on_the_batch(cuda_device):
     """A prompt alone, among others, and continued from a prefix: the same bits."""
     dev, hd = cuda_device, 128

@@ -12,6 +12,7 @@
 // codes of V become fp16 by byte permutes onto 1024 + 128 + c).  The layout is built around bytes in flight and
 // few instructions: 16 keys are the M of one tensor-core step, so the 8 columns carry up to 8 query heads,
 //     S^T[key][head] = K . Q^T,          O^T[dim][head] += V^T . P^T,
+// (a larger group reads its keys once for every 8)
 // and the k indices of S and the dims of O are permuted so that each thread needs whole 16-byte
 // runs of the codes.  Each warp has a ring of its own (cp.async, whole runs of a page: copies that took 32 bytes
 // of a row at a time moved 1.5 times the bytes from L2), so the loop has no barrier: a warp waits for its copies only.
