@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float il = l > 0.f || l != l ? 1.f / l : 0.f;
                 const bool mine = r < toks * G;
                 T* row = static_cast<T*>(p.out) + ((int64_t)(w.q0 + tok) * p.n_heads + w.kvh * G + r % G) * HD;
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                     float o[32];
                     if (nt > 0) {
