@@ -417,8 +417,9 @@ TPTC_API int tptc_kv8_attn(const tptc_kv8* cache, int type, const void* d_q, int
  * d_cu_q[b] .. d_cu_q[b + 1] of n_q and the keys d_cu_k[b] .. d_cu_k[b + 1] of n_k; its queries are the last
  * of its key positions: query i of lq sees keys 0 .. lk - lq + i (a row that sees none gets
  * zeros).  Rows: token t at element t * stride, heads adjacent; 16-byte aligned, strides multiples
- * of 8 elements; d_out [n_q][n_heads][head_dim], 32-byte aligned.  Any n_heads that is a multiple of n_kv, up to 128 query heads per kv
- * head; head_dim 64, 96 or 128.  max_q: no sequence has more query rows.  d_out overlaps no input.  K and V hold finite
+ * of 8 elements; d_out [n_q][n_heads][head_dim], 32-byte aligned, overlaps no input.  Any n_heads
+ * that is a multiple of n_kv, up to 128 query heads per kv head; head_dim 64, 96 or 128.  max_q:
+ * no sequence has more query rows.  K and V hold finite
  * values (what lies behind the last key of a sequence is never used). */
 TPTC_API int tptc_attn_packed(int type, const void* d_q, int64_t q_stride, const void* d_k, int64_t k_stride,
                               const void* d_v, int64_t v_stride, void* d_out, const int32_t* d_cu_q,
