@@ -326,29 +326,30 @@ def _own(s):
     c = s["c"]
     kind = {"f32": K.F32, "f16": K.F16, "bf16": K.BF16}[c["type"]]
     t = TYPES[c["type"]]
+    st = torch.cuda.current_stream().cuda_stream  # the one that the inputs and the outputs belong to
     if c["op"] == "logprobs":
         r, n = c["rows"], c["n_top"]
         logprob, entropy = torch.empty(2, r, device=DEV).unbind(0)
         top_lp, top_ids = torch.empty(r, n, device=DEV), torch.empty(r, n, dtype=torch.int32, device=DEV)
-        K.logprobs(s["logits"], kind, r, c["vocab"], c["vocab"], s["tokens"], logprob, entropy, n, top_ids, top_lp)
+        K.logprobs(s["logits"], kind, r, c["vocab"], c["vocab"], s["tokens"], logprob, entropy, n, top_ids, top_lp, stream=st)
         return dict(logprob=logprob, entropy=entropy, top_ids=top_ids, top_logprobs=top_lp)
     kv, hd = c["n_kv"], c["hd"]
     if c["op"] == "prompt":
         h, out = c["n_heads"], torch.empty_like(s["q"])
         K.attn_packed(s["q"], s["k"], s["v"], out, kind, h * hd, kv * hd, kv * hd, s["cu"], s["cu"], c["n_seq"], s["total"],
-                      s["total"], s["most"], h, kv, hd)
+                      s["total"], s["most"], h, kv, hd, stream=st)
         return out
     cache = _handle(s, K)
     if c["op"] == "decode":
         h, out = c["n_heads"], torch.empty_like(s["q"])
         if "work" not in s:
             s["work"] = torch.zeros(cache.attn_workspace_bytes(h), dtype=torch.uint8, device=DEV)
-        cache.attn(s["q"], h * hd, kind, s["lens"], h, out, s["work"], s["work"].numel())
+        cache.attn(s["q"], h * hd, kind, s["lens"], h, out, s["work"], s["work"].numel(), stream=st)
         return out
 
     def read(cu, start, total, most, kind, t):
         k, v = torch.empty(2, total, kv, hd, dtype=t, device=DEV).unbind(0)
-        cache.read(cu, start, total, most, kind, k, v)
+        cache.read(cu, start, total, most, kind, k, v, stream=st)
         return k, v
 
     if c["op"] == "read":
@@ -360,7 +361,7 @@ def _own(s):
     k = torch.empty(s["total"], kv, hd, dtype=t, device=DEV)
     qkv, e = s["qkv"].data_ptr(), s["qkv"].element_size() * hd
     cache.append(s["rope"], kind, qkv, width, qkv + h * e, width, qkv + (h + kv) * e, width, h, q, k, s["cu"], s["start"],
-                 s["total"], s["most"])
+                 s["total"], s["most"], stream=st)
     if c["type"] == "f32":
         kind, t = K.F16, torch.float16
     ck, cv = read(s["back_cu"], s["back_start"], s["back_total"], s["back_most"], kind, t)
