@@ -144,7 +144,7 @@ class Kv8Cache:
     def __init__(self, d_k, d_v, d_k_scale, d_v_scale, d_table, d_status, n_pages: int, page: int, n_kv: int,
                  head_dim: int, n_seq: int, max_pages: int):
         self._keep = (d_k, d_v, d_k_scale, d_v_scale, d_table, d_status)
-        self._c = Kv8C(_ptr(d_k), _ptr(d_v), _ptr(d_k_scale), _ptr(d_v_scale), _ptr(d_table), _opt(d_status), n_pages,
+        self._c = Kv8C(_ptr(d_k), _ptr(d_v), _ptr(d_k_scale), _ptr(d_v_scale), _opt(d_table), _opt(d_status), n_pages,
                        page, n_kv, head_dim, n_seq, max_pages)
         self._h = ctypes.addressof(self._c)
 
@@ -152,14 +152,14 @@ class Kv8Cache:
                n_heads: int, d_q_out, d_k_out, d_cu, d_start, n_tokens: int, max_new: int,
                stream: Optional[int] = None) -> None:
         """New keys and values of a ragged batch into the cache, rotated on the way with q (tptc_kv8_append)."""
-        check(lib().tptc_kv8_append(self._h, None if rope is None else rope._h, type_, _opt(d_q), q_stride, _ptr(d_k),
-                                    k_stride, _ptr(d_v), v_stride, n_heads, _opt(d_q_out), _opt(d_k_out), _ptr(d_cu),
-                                    _ptr(d_start), n_tokens, max_new, stream))
+        check(lib().tptc_kv8_append(self._h, None if rope is None else rope._h, type_, _opt(d_q), q_stride, _opt(d_k),
+                                    k_stride, _opt(d_v), v_stride, n_heads, _opt(d_q_out), _opt(d_k_out), _opt(d_cu),
+                                    _opt(d_start), n_tokens, max_new, stream))
 
     def read(self, d_cu, d_start, n_tokens: int, max_rows: int, type_: int, d_k_out, d_v_out,
              stream: Optional[int] = None) -> None:
         """The values of ranges of positions as packed dense rows (tptc_kv8_read)."""
-        check(lib().tptc_kv8_read(self._h, type_, _ptr(d_cu), _ptr(d_start), n_tokens, max_rows, _opt(d_k_out),
+        check(lib().tptc_kv8_read(self._h, type_, _opt(d_cu), _opt(d_start), n_tokens, max_rows, _opt(d_k_out),
                                   _opt(d_v_out), stream))
 
     def attn_workspace_bytes(self, n_heads: int) -> int:
@@ -168,21 +168,21 @@ class Kv8Cache:
     def attn(self, d_q, q_stride: int, type_: int, d_len, n_heads: int, d_out, d_workspace, workspace_bytes: int,
              stream: Optional[int] = None) -> None:
         """Attention of one query row per sequence over its first d_len[b] positions (tptc_kv8_attn)."""
-        check(lib().tptc_kv8_attn(self._h, type_, _ptr(d_q), q_stride, _ptr(d_len), n_heads, _ptr(d_out),
-                                  _ptr(d_workspace), workspace_bytes, stream))
+        check(lib().tptc_kv8_attn(self._h, type_, _opt(d_q), q_stride, _opt(d_len), n_heads, _opt(d_out),
+                                  _opt(d_workspace), workspace_bytes, stream))
 
 
 def attn_packed(d_q, d_k, d_v, d_out, type_: int, q_stride: int, k_stride: int, v_stride: int, d_cu_q, d_cu_k, n_seq: int,
                 n_q: int, n_k: int, max_q: int, n_heads: int, n_kv: int, head_dim: int, d_status=None,
                 stream: Optional[int] = None) -> None:
     """Causal attention over packed prompts; queries are the last of their sequence's keys (tptc_attn_packed)."""
-    check(lib().tptc_attn_packed(type_, _ptr(d_q), q_stride, _ptr(d_k), k_stride, _ptr(d_v), v_stride, _ptr(d_out),
-                                 _ptr(d_cu_q), _ptr(d_cu_k), n_seq, n_q, n_k, max_q, n_heads, n_kv, head_dim,
+    check(lib().tptc_attn_packed(type_, _opt(d_q), q_stride, _opt(d_k), k_stride, _opt(d_v), v_stride, _opt(d_out),
+                                 _opt(d_cu_q), _opt(d_cu_k), n_seq, n_q, n_k, max_q, n_heads, n_kv, head_dim,
                                  _opt(d_status), stream))
 
 
 def logprobs(d_logits, type_: int, rows: int, vocab: int, row_stride: int, d_token, d_logprob, d_entropy, n_top: int,
              d_top_id, d_top_logprob, stream: Optional[int] = None) -> None:
     """Log probabilities of given tokens, entropy and the n_top largest of each row (tptc_logprobs)."""
-    check(lib().tptc_logprobs(type_, _ptr(d_logits), rows, vocab, row_stride, _opt(d_token), _opt(d_logprob),
+    check(lib().tptc_logprobs(type_, _opt(d_logits), rows, vocab, row_stride, _opt(d_token), _opt(d_logprob),
                               _opt(d_entropy), n_top, _opt(d_top_id), _opt(d_top_logprob), stream))
