@@ -380,7 +380,8 @@ typedef struct {
  *     adjacent (n_heads x head_dim, n_kv x head_dim): slices of a fused projection fit.  16-byte
  *     aligned, strides multiples of 16 bytes.  d_q and n_heads may be NULL and 0.
  *   d_q_out, d_k_out: the rotated rows, contiguous, of `type`; each may be NULL (not wanted).
- *     d_q_out may be d_q itself, and d_k_out d_k, where the stride leaves no gap.
+ *     d_q_out may be d_q itself, and d_k_out d_k, where the stride leaves no gap (refused where it
+ *     does); otherwise the outputs overlap neither an input nor one another.
  *   rope: NULL stores and copies without rotating.
  * One scale per (page, kv head): with a the largest magnitude of the new rows in the page,
  * s = max(s_old, a * (1/127)), where s_old counts only if earlier positions of the sequence lie in the

@@ -29,7 +29,7 @@ def built_libs():
 
 # Modules that call entry points with made-up device addresses to see them refused.  A refusal that went
 # missing would launch a kernel on those addresses, so they run only where there is no GPU to launch on.
-NO_GPU_ONLY = {"test_serve_args", "test_serve_null"}
+NO_GPU_ONLY = {"test_serve_args", "test_serve_null", "test_serve_refusals"}
 
 
 @pytest.fixture(autouse=True)

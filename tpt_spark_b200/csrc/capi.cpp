@@ -642,6 +642,10 @@ TPTC_API int tptc_kv8_append(const tptc_kv8* cache, const tptc_rope* rope, int t
         if (bad_rows(d_q, q_stride, (int64_t)n_heads * hd, type) || misaligned(d_q_out, 16))
             return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: q rows must be 16-byte aligned and not overlap");
     }
+    // a contiguous row written in place of a strided one lies across other rows that are still to be read
+    if (n_tokens > 1 && ((d_q_out && d_q_out == d_q && q_stride != (int64_t)n_heads * hd) ||
+                         (d_k_out && d_k_out == d_k && k_stride != (int64_t)cache->n_kv * hd)))
+        return fail_code(nullptr, TPTC_ERR_ARG, "kv8_append: rows with gaps cannot be rotated in place");
     if (rope && (!rope->cos || !rope->sin || misaligned(rope->cos, 16) || misaligned(rope->sin, 16) || rope->rows <= 0 ||
                  rope->dim <= 0 || rope->dim % 16 || rope->dim > hd))
         return fail_code(nullptr, TPTC_ERR_ARG,
