@@ -408,7 +408,8 @@ TPTC_API int tptc_kv8_read(const tptc_kv8* cache, int type, const int32_t* d_cu,
  *     kv head h / (n_heads / n_kv).  A sequence of length 0 gets zeros.
  * d_workspace holds tptc_kv8_attn_workspace_bytes() bytes (for the current device) and must be zero
  * before its first use; each call leaves it ready for the next, of any shape that it is large
- * enough for.  Calls that may overlap on the GPU need separate workspaces.  Results do not
+ * enough for.  32 sequences (all, where there are fewer) of max_pages pages have less than 2^35 - 2^13
+ * positions together.  Calls that may overlap on the GPU need separate workspaces.  Results do not
  * depend on scheduling.  A length out of range gives zeros, a page id out of range NaN (with *status). */
 TPTC_API int64_t tptc_kv8_attn_workspace_bytes(const tptc_kv8* cache, int n_heads);
 TPTC_API int tptc_kv8_attn(const tptc_kv8* cache, int type, const void* d_q, int64_t q_stride, const int32_t* d_len,

@@ -29,3 +29,15 @@ def test_rotation_in_place_of_rows_with_gaps(kw):
              d_k_out=None, d_cu=P, d_start=P, n_tokens=4, max_new=4)
     a.update(kw)
     refused("in place", cache().append, **a)
+
+
+def test_attention_over_more_positions_than_its_sums_hold():
+    """A sequence of 2^30 positions is 2^26 tiles of 16 keys; 32 of them pass 31 bits, 31 do not."""
+    a = dict(d_q=P, q_stride=256, type_=K.F16, d_len=P, n_heads=4, d_out=P, d_workspace=P, workspace_bytes=1 << 30)
+    for c in (cache(n_seq=32, max_pages=1 << 26), cache(n_seq=900, max_pages=1 << 24, page=64), cache(n_seq=16, max_pages=(1 << 27) - 1)):
+        refused("positions", c.attn, **a)
+        refused("positions", c.attn_workspace_bytes, 4)
+    for c in (cache(n_seq=31, max_pages=1 << 26), cache(n_seq=900, max_pages=1 << 25), cache(n_seq=15, max_pages=(1 << 27) - 1)):
+        with pytest.raises(EngineError) as e:  # no GPU here: that is as far as an accepted call gets
+            c.attn_workspace_bytes(4)
+        assert e.value.code != ARG

@@ -697,6 +697,8 @@ static int kv8_attn_args(const tptc_kv8* c, int type, int n_heads) {
     if (n_heads <= 0 || n_heads % c->n_kv)
         return fail_code(nullptr, TPTC_ERR_ARG, "kv8_attn: n_heads must be a positive multiple of n_kv");
     if ((int64_t)c->n_seq * n_heads > INT32_MAX) return fail_code(nullptr, TPTC_ERR_ARG, "kv8_attn: too many sequences");
+    if (!tptc::kv8_attn_fits(*c))
+        return fail_code(nullptr, TPTC_ERR_ARG, "kv8_attn: too many positions in 32 sequences of max_pages pages");
     return TPTC_OK;
 }
 

@@ -677,6 +677,12 @@ cudaError_t init_t() {
 
 }  // namespace
 
+// A warp adds the units of up to 32 sequences in 32 bits.
+bool kv8_attn_fits(const tptc_kv8& c) {
+    const int64_t most = (int64_t)c.max_pages * c.page / kTile + kSetup;
+    return std::min(c.n_seq, 32) * most <= INT32_MAX;
+}
+
 size_t kv8_attn_workspace(const tptc_kv8& c, int n_heads, int sms) {
     return record_bytes(sms) + (size_t)c.n_seq * pairs_of(n_heads, c.n_kv) * sizeof(int);
 }

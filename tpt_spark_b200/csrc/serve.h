@@ -110,6 +110,7 @@ struct Kv8Attn {
     void* out;
     uint8_t* workspace;  // kv8_attn_workspace() bytes; the counters at its end are zero between calls
 };
+bool kv8_attn_fits(const tptc_kv8& c);  // whether the kernel's sums hold the longest batch that the table allows
 size_t kv8_attn_workspace(const tptc_kv8& c, int n_heads, int sms);
 cudaError_t launch_kv8_attn(int type, const Kv8Attn& a, int sms, cudaStream_t st);
 cudaError_t kv8_attn_init_device();
