@@ -354,7 +354,7 @@ TPTC_API int tptc_attn_decode_noalloc_status(void* stream, int* out_code);
 typedef struct {
     int8_t* k;             /* [n_pages][n_kv][page][head_dim] codes in -127..127, 16-byte aligned */
     int8_t* v;             /* the same for V */
-    float* k_scale;        /* [n_pages][n_kv] */
+    float* k_scale;        /* [n_pages][n_kv], not negative and finite, or NaN (see tptc_kv8_append) */
     float* v_scale;
     const int32_t* table;  /* [n_seq][max_pages] page ids: position i of sequence b lies in page
                               table[b][i / page], row i % page */

@@ -231,3 +231,23 @@ def test_two_streams_and_graphs(cuda_device):
     torch.cuda.synchronize()
     for out, w in zip(outs, want):
         assert torch.equal(out, w)
+
+
+@pytest.mark.parametrize("kind", [K.F16, K.BF16, K.F32])
+def test_scales_below_the_normal_range(cuda_device, kind):
+    """A cache that the caller filled may hold a page whose scale is subnormal: its values are next to nothing."""
+    lens, hd = [60, 20], 64
+    c = Cache(lens, 16, 2, hd, 21)
+    p = c.table[0].long()
+    c.vs[p[0]], c.vs[p[2]] = 1e-40, 2.0 ** -149  # the first page, and one behind a normal one
+    c.ks[p[2]] = 1e-40
+    c.vs[c.table[1, :2].long()] = 1e-40          # a sequence of nothing else
+    c.handle = c.to(cuda_device)
+    q = (0.7 * torch.randn(2, 4, hd, generator=torch.Generator().manual_seed(22))).to(TYPES[kind])
+    got = run(c, q.to(cuda_device), kind, lens, cuda_device)
+    check(got, reference(c, q, lens), c, lens, kind)
+    # the last is below 127e-40.  fp16: zeros.  bf16, f32: weights as above (2^-10.5 + 2^-16); 2^-126 / l with a sum l of
+    # 20 weights of at most 2^8 has steps of 2^-149 (2^-11 relative); the outputs' own steps are 2^-133 and 2^-149
+    want = reference(c, q, lens)[1]
+    tol = 0 if kind == K.F16 else 2.0 ** -9 * 127e-40 + 2.0 ** -133
+    assert ((got[1].cpu().double() - want).abs() <= tol + (kind == K.F16) * want.abs()).all()

@@ -435,14 +435,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
                     c0 = fmaxf(c0, __shfl_xor_sync(0xffffffffu, c0, d));
                     c1 = fmaxf(c1, __shfl_xor_sync(0xffffffffu, c1, d));
                 }
-                const float lv = lg2(vs);
+                // (log2 of a scale of zero or below the normal range would be -inf, and its weights inf or NaN)
+                const float lv = lg2(fmaxf(vs, 1.17549435e-38f));
                 auto move = [&](float c, float& m, float& l, float& r, float& w, float& v) {
                     const float mn = fmaxf(m, c), rn = fmaxf(r, c + lv);
                     l *= m == mn ? 1.f : ex2(m - mn);
                     const float beta = r == rn ? 1.f : ex2(r - rn);
                     m = mn, r = rn;
                     w = rn == -INFINITY ? INFINITY : ex2(fminf(mn - rn, 127.f));
-                    v = vs == 0.f ? 0.f : vs * w;
+                    v = vs * w;
                     return beta;
                 };
                 const float b0 = move(c0, m0, l0, r0, w0, v0), b1 = move(c1, m1, l1, r1, w1, v1);
