@@ -187,3 +187,29 @@ def test_in_a_graph_on_another_stream(cuda_device):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+# scores as q . k, their first two dims: (the queries' values, the keys' values by index)
+FAR = {
+    "alike": lambda i, big: ((big, 0), (i * 0 + big, i * 0)),
+    "alike below zero": lambda i, big: ((big, 0), (i * 0 - big, i * 0)),
+    "climbing": lambda i, big: ((big, 0), (big / 2 + i % 900 * (big / 2048), i * 0)),
+    "falling": lambda i, big: ((big, 0), (big - i % 900 * (big / 2048), i * 0)),
+    "apart by f32 steps": lambda i, big: ((60000, 1), (i * 0 + 60000, i * 7919 % 4 * 256)),
+    "apart by little": lambda i, big: ((2048, 1), (i * 0 + 4096, i * 7919 % 9)),
+}
+
+
+@pytest.mark.parametrize("what", FAR)
+@pytest.mark.parametrize("kind,big", [(K.F16, 32768), (K.F16, 60000), (K.BF16, 57344), (K.BF16, 2.0 ** 60)])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+def test_scores_far_from_zero(cuda_device, hd, kind, big, what):
+    """Finite inputs whose scores times log2 e / sqrt(hd) have f32 steps far above 1; the scores themselves are exact."""
+    n = 700
+    (qa, qb), (ka, kb) = FAR[what](torch.arange(n, dtype=torch.float64), big)
+    g = torch.Generator().manual_seed(5)
+    q, k, v = torch.zeros(n, 2, hd), torch.zeros(n, 1, hd), torch.randn(n, 1, hd, generator=g).to(TYPES[kind])
+    q[..., 0], q[..., 1], k[:, 0, 0], k[:, 0, 1] = qa, qb, ka, kb
+    q, k = q.to(TYPES[kind]), k.to(TYPES[kind])
+    got = run(q.to(cuda_device), k.to(cuda_device), v.to(cuda_device), kind, [n], [n], cuda_device)
+    check(got, reference(q, k, v, [n], [n]), v, kind)
