@@ -422,7 +422,10 @@ TPTC_API int tptc_kv8_attn(const tptc_kv8* cache, int type, const void* d_q, int
  * of 8 elements; d_out [n_q][n_heads][head_dim], 32-byte aligned, overlaps no input.  Any n_heads
  * that is a multiple of n_kv, up to 128 query heads per kv head; head_dim 64, 96 or 128.  max_q:
  * no sequence has more query rows.  K and V hold finite
- * values (what lies behind the last key of a sequence is never used). */
+ * values (what lies behind the last key of a sequence is never used).
+ *   d_status: device word, zero at first, may be NULL; receives TPTC_ERR_ARG (offsets out of range: the sequence's rows
+ *     are not written) or TPTC_ERR_TIMEOUT (a wait inside the kernel gave up, about 17 s after its work stood
+ *     still: rows may be unwritten).  Without it neither is reported. */
 TPTC_API int tptc_attn_packed(int type, const void* d_q, int64_t q_stride, const void* d_k, int64_t k_stride,
                               const void* d_v, int64_t v_stride, void* d_out, const int32_t* d_cu_q,
                               const int32_t* d_cu_k, int n_seq, int n_q, int n_k, int max_q, int n_heads, int n_kv,

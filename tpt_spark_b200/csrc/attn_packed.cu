@@ -83,23 +83,31 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, u
         : "memory");
 }
 
-// Waits for a phase of a barrier; false, with the status set, when it does not come (a bounded number
-// of polls).  One instruction and a branch where the phase is complete: the loops of this kernel wait
-// up to ten times per tile, and with a called-out abort flag and a vote in each wait 8192 tokens took
-// 523 us instead of 463.  A poll may sleep for 10 us, so that waiting warps leave the issue slots to the others.
+// Waits for a phase of a barrier; false when it does not come (a bounded number
+// of polls) or when another wait of the CTA gave up.  One instruction and a branch where the phase is complete:
+// the loops of this kernel wait up to ten times per tile, and with a called-out abort flag and a vote in each
+// wait 8192 tokens took 523 us instead of 463; the flag is read behind a poll that failed.  Such a poll sleeps
+// for 4 us (measured), so that waiting warps leave the issue slots to the others, and the limit is 17 s: the longest
+// wait is one item, and the keys that fit the memory take 10.
 constexpr uint32_t kPolls = 1u << 22;
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, int32_t* status) {
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, const uint32_t* gave_up) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n .reg .u32 n;\n mov.u32 n, %3;\n"
+        "{\n .reg .pred p;\n .reg .u32 n, g;\n mov.u32 n, %3;\n"
         "POLL:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n @p bra DONE;\n"
-        " sub.u32 n, n, 1;\n setp.eq.u32 p, n, 0;\n @!p bra POLL;\n setp.ne.u32 p, n, 0;\n"
+        " sub.u32 n, n, 1;\n ld.volatile.shared.u32 g, [%5];\n setp.eq.u32 p, n, 0;\n setp.ne.or.u32 p, g, 0, p;\n @!p bra POLL;\n"
+        " setp.lt.u32 p, n, 0;\n"
         "DONE:\n selp.u32 %0, 1, 0, p;\n}\n"
         : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "n"(kPolls), "r"(10000)
+        : "r"(smem_u32(bar)), "r"(parity), "n"(kPolls), "r"(10000), "r"(smem_u32(gave_up))
         : "memory");
-    if (!ok && status) atomicExch(status, TPTC_ERR_TIMEOUT);
     return ok != 0;
+}
+// The same for what writes to this CTA's memory or reads it, and so has to end before the CTA does, whoever gave up.
+__device__ __forceinline__ bool wait_own(uint64_t* bar, uint32_t parity) {
+    for (uint32_t n = 0; n < kPolls; n++)
+        if (mbar_try_wait(bar, parity)) return true;
+    return false;
 }
 
 // One lane of a converged warp.  (The compiler keeps what a warp computes alike in uniform registers, where
@@ -336,11 +344,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint4 response;
     __shared__ Item items[2];
     __shared__ int counts[kSeqs];
-    __shared__ uint32_t tmem_slot;
+    __shared__ uint32_t tmem_slot, gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = p.n_heads / p.n_kv;
 
     if (threadIdx.x == 0) {
+        gave_up = 0;
         mbar_init(&q_full, 1);
         mbar_init(&q_empty, 2);  // both tiles' products are through with it
         for (int s = 0; s < S; s++) {
@@ -394,7 +403,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_phase(bar, parity, p.status); };
+    auto give_up = [&] {
+        *reinterpret_cast<volatile uint32_t*>(&gave_up) = 1;
+        if (p.status) atomicExch(p.status, TPTC_ERR_TIMEOUT);
+        return false;
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_phase(bar, parity, &gave_up) || give_up(); };
     // the n-th item of the CTA, for a lane (copies) or a warp; false: no more
     auto get_item = [&](int n, Item& w, bool whole_warp) {
         const int s = n & 1;
@@ -414,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int n = 0; ok && get_item(n, w, false); n++) {
                 if (w.ntot <= kLead) mbar_arrive(&wanted);
                 if (w.ntot == 0) continue;
-                if (nq > 0) ok = mbar_wait_backoff(&q_empty, (nq - 1) & 1, p.status);
+                if (nq > 0) ok = mbar_wait_backoff(&q_empty, (nq - 1) & 1, nullptr) || give_up();
                 if (!ok) break;
                 nq++;
                 mbar_expect_tx(&q_full, (w.toks[1] > 0 ? 2 : 1) * ((uint32_t)(p.tokens * G) * 128 * L::NC));
@@ -426,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 for (int k = 0; k < 2 * w.ntot; k++, i0++) {
                     const int s = i0 % S;
-                    if (i0 >= S) ok = mbar_wait_backoff(&empty[s], ((i0 / S) - 1) & 1, p.status);
+                    if (i0 >= S) ok = mbar_wait_backoff(&empty[s], ((i0 / S) - 1) & 1, nullptr) || give_up();
                     if (!ok) break;
                     mbar_expect_tx(&full[s], L::kTile);
 #pragma unroll
@@ -437,8 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             // the copies still in flight land before the CTA exits
-            if (nq > 0) wait_phase(&q_full, (nq - 1) & 1, nullptr);
-            for (int k = i0 > S ? i0 - S : 0; k < i0; k++) wait_phase(&full[k % S], (k / S) & 1, nullptr);
+            if (nq > 0) wait_own(&q_full, (nq - 1) & 1);
+            for (int k = i0 > S ? i0 - S : 0; k < i0; k++) wait_own(&full[k % S], (k / S) & 1);
         }
         if (warp == 3) {  // the items behind the first, asked for when the copies of the one before near their end
             if (lane == 0) mbar_arrive(&item_full[0]);
@@ -449,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 at.k = -1;
                 if (wait(&wanted, (n - 1) & 1)) do {  // (indices behind the list's end are taken over until none is left)
                     if (lane == 0) request_item(&response, &taken);
-                    if (wait(&taken, asked++ & 1)) at = taken_place(&response);
+                    if (wait_own(&taken, asked++ & 1) || give_up()) at = taken_place(&response);
                     else at.k = -1;
                     fence_proxy_async_smem();  // read before the slot is written again
                     __syncwarp();
@@ -534,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // every product issued has completed before TMEM is freed
             commit(&drain[t]);
-            wait_phase(&drain[t], 0, nullptr);
+            wait_own(&drain[t], 0);
             __syncwarp();
         }
     } else {  // one thread per lane of tile A or B
