@@ -65,3 +65,43 @@ def attend(q, k, v, limit):
         p = torch.softmax(s.masked_fill(~seen, -math.inf)[some], 1)
         out[some, h] = p @ v[:, h // G]
     return out
+
+
+def attend_and_noise(q, k, v, limit, drop=None):
+    """attend(), and for each (row, head) sum p_j^2 |v_j|^2, what independent errors of the weights act on.
+    drop: a slice of keys that is left out of the sums, as a kernel that lost them would."""
+    H, G = q.shape[1], q.shape[1] // k.shape[1]
+    out, noise = torch.zeros_like(q), torch.zeros(q.shape[:2], dtype=q.dtype)
+    seen = torch.arange(k.shape[0])[None] < limit[:, None]
+    if drop is not None:
+        seen[:, drop] = False
+    for h in range(H):
+        s = (q[:, h] @ k[:, h // G].T / math.sqrt(q.shape[2])).masked_fill(~seen, -math.inf)
+        p = torch.softmax(s, 1).nan_to_num(0.0)
+        out[:, h], noise[:, h] = p @ v[:, h // G], p ** 2 @ (v[:, h // G] ** 2).sum(1)
+    return out, noise
+
+
+def norm_bound(want, noise, weight, result):
+    """How far a (row, head) of attention may lie from `want`, as a norm over head_dim: the weights carry independent
+    roundings of up to `weight` relative (their mean square is at most a third of its square) and the output's
+    elements of up to `result`; three times the root of the two together, as the sum of two or more roundings stays
+    below sqrt(6) of it and that of many has nearly its mean.  f32 sums, exponentials and scores: 2^-16 of the same sizes."""
+    size = want.norm(dim=-1)
+    return 3 * ((weight ** 2 * noise + result ** 2 * size ** 2) / 3).sqrt() + 2.0 ** -16 * (size + noise.sqrt()) + 1e-9
+
+
+def whole_inputs(case, dtype):
+    """Cache and queries (scores within a few units) for the cases that look for lost keys."""
+    n_heads, n_kv, hd, page, lens = case
+    c = Cache(lens, page, n_kv, hd, 23)
+    q = (0.7 * torch.randn(len(lens), n_heads, hd, generator=torch.Generator().manual_seed(24))).to(dtype)
+    return c, q
+
+
+def roundings(dtype):
+    """Of the weights and of the result in decode attention: 16-bit queries take fp16 weights, f32 ones two fp16 parts
+    (scores of up to 2^5 carry 2^-22 each: 2^-17)."""
+    if dtype == torch.float32:
+        return 2.0 ** -17, 2.0 ** -24
+    return 2.0 ** -11, torch.finfo(dtype).eps / 2

@@ -3,7 +3,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from kv8_ref import TYPES, attend  # noqa: E402
+from kv8_ref import TYPES, attend, attend_and_noise, norm_bound  # noqa: E402
 from tpt_spark_b200 import kernels as K  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -213,3 +213,17 @@ def test_scores_far_from_zero(cuda_device, hd, kind, big, what):
     q, k = q.to(TYPES[kind]), k.to(TYPES[kind])
     got = run(q.to(cuda_device), k.to(cuda_device), v.to(cuda_device), kind, [n], [n], cuda_device)
     check(got, reference(q, k, v, [n], [n]), v, kind)
+
+
+@pytest.mark.parametrize("kind", [K.F16, K.BF16])
+@pytest.mark.parametrize("H,n_kv,hd,lq,lk", [(4, 1, 128, 3000, 3000), (3, 1, 64, 400, 5000), (2, 2, 96, 1500, 1500)])
+def test_no_key_is_lost(cuda_device, kind, H, n_kv, hd, lq, lk):
+    """Each row's output by its norm, which a few missing keys would exceed (shown in test_serve_bounds.py)."""
+    g = torch.Generator().manual_seed(6)
+    q, k, v = (torch.randn(n, h, hd, generator=g).to(TYPES[kind]) for n, h in ((lq, H), (lk, n_kv), (lk, n_kv)))
+    got = run(q.to(cuda_device), k.to(cuda_device), v.to(cuda_device), kind, [lq], [lk], cuda_device)
+    want, noise = attend_and_noise(q.double(), k.double(), v.double(), limits(lq, lk))
+    eps = torch.finfo(TYPES[kind]).eps / 2
+    err = (got.cpu().double() - want).norm(dim=-1)
+    bound = norm_bound(want, noise, eps, eps)
+    assert (err <= bound).all(), (int((err / bound).max(1)[0].argmax()), float((err / bound).max()))

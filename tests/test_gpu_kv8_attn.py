@@ -3,7 +3,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from kv8_ref import TYPES, Cache, attend  # noqa: E402
+from kv8_ref import TYPES, Cache, attend, attend_and_noise, norm_bound, roundings, whole_inputs  # noqa: E402
 from tpt_spark_b200 import kernels as K  # noqa: E402
 from tpt_spark_b200._lib import EngineError  # noqa: E402
 
@@ -251,3 +251,28 @@ def test_scales_below_the_normal_range(cuda_device, kind):
     want = reference(c, q, lens)[1]
     tol = 0 if kind == K.F16 else 2.0 ** -9 * 127e-40 + 2.0 ** -133
     assert ((got[1].cpu().double() - want).abs() <= tol + (kind == K.F16) * want.abs()).all()
+
+
+WHOLE = [
+    # n_heads, n_kv, hd, page, lens
+    (2, 1, 128, 16, [40000]),
+    (8, 1, 64, 16, [5000, 300]),
+    (32, 8, 128, 64, [1000, 2777]),
+    (12, 4, 96, 32, [47, 1025]),
+]
+
+
+@pytest.mark.parametrize("kind", [K.F32, K.F16, K.BF16])
+@pytest.mark.parametrize("case", WHOLE, ids=[str(i) for i in range(len(WHOLE))])
+def test_no_tile_is_lost(cuda_device, case, kind):
+    """Each head's output by its norm, which a missing tile of 16 keys or a missing part of a join would exceed (shown for
+    the same cases in test_serve_bounds.py)."""
+    n_heads, n_kv, hd, page, lens = case
+    c, q = whole_inputs(case, TYPES[kind])
+    c.handle = c.to(cuda_device)
+    got = run(c, q.to(cuda_device), kind, lens, cuda_device)
+    for b, n in enumerate(lens):
+        k, v = c.values(b, n)
+        want, noise = attend_and_noise(q[b:b + 1].double(), k, v, torch.tensor([n]))
+        err = (got[b:b + 1].cpu().double() - want).norm(dim=-1)
+        assert (err <= norm_bound(want, noise, *roundings(TYPES[kind]))).all(), (b, err)
