@@ -386,7 +386,9 @@ typedef struct {
  * One scale per (page, kv head): with a the largest magnitude of the new rows in the page,
  * s = max(s_old, a * (1/127)), where s_old counts only if earlier positions of the sequence lie in the
  * page; a new code is x * (1 / s) rounded to nearest even, and where s grows the earlier codes c become c * s_old / s,
- * rounded.  A scale below the smallest normal float is 0.  A page that receives a value that is
+ * rounded.  A value is thus off by at most half of the scale that it was stored with and half of s for each time the
+ * scale has grown since: s / 2 for rows that come together, (1 + growths) s / 2 in a page that
+ * fills row by row.  A scale below the smallest normal float is 0.  A page that receives a value that is
  * not finite gets scale NaN, so whatever attends to it becomes NaN.  Rows of the page behind
  * the last new position keep their codes.  No two sequences of one call may append to the same page.
  * max_new: no sequence brings more new rows (n_tokens in all). */
@@ -397,7 +399,9 @@ TPTC_API int tptc_kv8_append(const tptc_kv8* cache, const tptc_rope* rope, int t
 
 /* The values that positions d_start[b] .. of each sequence stand for, as packed rows [n_tokens][n_kv][head_dim]
  * of `type` (code * scale in f32, rounded once): the K and V that tptc_attn_packed takes to
- * continue a cached prefix.  Either output may be NULL. */
+ * continue a cached prefix.  Either output may be NULL.  Rows of a page id outside the cache are not written.
+ * A page whose scale is NaN reads as NaN, which tptc_attn_packed does not take: it may spread to any row of
+ * that sequence (of no other), where tptc_kv8_attn confines it to the heads and lengths that reach the page. */
 TPTC_API int tptc_kv8_read(const tptc_kv8* cache, int type, const int32_t* d_cu, const int32_t* d_start,
                            int n_tokens, int max_rows, void* d_k_out, void* d_v_out, void* stream);
 
@@ -405,7 +409,8 @@ TPTC_API int tptc_kv8_read(const tptc_kv8* cache, int type, const int32_t* d_cu,
  * step of a batch; append the step's key and value first).
  *   d_q: rotated queries of `type`, sequence b at element b * q_stride, [n_heads][head_dim];
  *   d_out: [n_seq][n_heads][head_dim] of `type` = softmax(q.k / sqrt(head_dim)) . V, query head h reading
- *     kv head h / (n_heads / n_kv).  A sequence of length 0 gets zeros.
+ *     kv head h / (n_heads / n_kv).  A sequence of length 0 gets zeros.  Queries count in steps of 2^-16 (f32: 2^-23)
+ *     of the largest element of their head; the weights of V are rounded to fp16 (f32: two fp16 parts); sums are f32.
  * d_workspace holds tptc_kv8_attn_workspace_bytes() bytes (for the current device) and must be zero
  * before its first use; each call leaves it ready for the next, of any shape that it is large
  * enough for.  32 sequences (all, where there are fewer) of max_pages pages have less than 2^35 - 2^13
@@ -421,7 +426,8 @@ TPTC_API int tptc_kv8_attn(const tptc_kv8* cache, int type, const void* d_q, int
  * zeros).  Rows: token t at element t * stride, heads adjacent; 16-byte aligned, strides multiples
  * of 8 elements; d_out [n_q][n_heads][head_dim], 32-byte aligned, overlaps no input.  Any n_heads
  * that is a multiple of n_kv, up to 128 query heads per kv head; head_dim 64, 96 or 128.  max_q:
- * no sequence has more query rows.  K and V hold finite
+ * no sequence has more query rows.  The weights of V are rounded to `type`; scores and sums are f32, and a row whose
+ * scores leave f32's range is NaN.  K and V hold finite
  * values (what lies behind the last key of a sequence is never used).
  *   d_status: device word, zero at first, may be NULL; receives TPTC_ERR_ARG (offsets out of range: the sequence's rows
  *     are not written) or TPTC_ERR_TIMEOUT (a wait inside the kernel gave up, about 17 s after its work stood

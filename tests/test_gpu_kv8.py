@@ -329,3 +329,43 @@ def test_on_a_stream_and_in_a_graph(cuda_device):
         graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(c.dev["k"], codes) and torch.equal(c.dev["vs"], scale) and torch.equal(out[0], out[1])
+
+
+@pytest.mark.parametrize("kind", [K.F32, K.BF16])
+@pytest.mark.parametrize("page", [16, 32, 64])
+def test_a_page_that_fills_row_by_row(cuda_device, page, kind):
+    """Against the values that went in: a row is rounded when it is stored and again each time the scale grows, by at most
+    half of the scale of that moment."""
+    dev, hd, n_kv = cuda_device, 128, 4
+    c = Cache([2 * page], page, n_kv, hd, seed=40)
+    cache = c.to(dev)
+    g = torch.Generator().manual_seed(41)
+    rows = torch.randn(2 * page, n_kv, hd, generator=g).to(TYPES[kind])
+    rows[page:] *= torch.linspace(0.2, 3.0, page)[:, None, None].to(TYPES[kind])  # the second page: it grows and grows
+    x, one = rows.to(dev), torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    bound = torch.zeros(2 * page, n_kv)
+    for i in range(2 * page):
+        p = int(c.table[0, i // page])
+        before = c.dev["vs"][p].cpu() if i % page else torch.zeros(n_kv)
+        cache.append(None, kind, None, 0, x[i], n_kv * hd, x[i], n_kv * hd, 0, None, None, one,
+                     torch.tensor([i], dtype=torch.int32, device=dev), 1, 1)
+        torch.cuda.synchronize()
+        now = c.dev["vs"][p].cpu()
+        grown = now > before
+        first = i - i % page
+        bound[first:i] += torch.where(grown, now, 0.0)  # the earlier rows, rounded again
+        bound[i] = now
+    # half a step each; the product with 1 / s and the quotient of scales: as for one append, 12 U of up to 127 steps
+    bound = bound.double() * (0.5 + 127 * 12 * U)
+    stored = [torch.stack([c.dev[n][int(c.table[0, i // page]), :, i % page] * c.dev[n + "s"][int(c.table[0, i // page])][:, None]
+                           for i in range(2 * page)]).cpu().double() for n in "kv"]
+    for got in stored:
+        assert ((got - rows.double()).abs().amax(2) <= bound).all()
+    # and with all rows at once half a step of the last scale
+    cache.append(None, kind, None, 0, x, n_kv * hd, x, n_kv * hd, 0, None, None, one * 2 * page,
+                 torch.zeros(1, dtype=torch.int32, device=dev), 2 * page, 2 * page)
+    out = torch.empty(2, 2 * page, n_kv, hd, device=dev)
+    cache.read(one * 2 * page, torch.zeros(1, dtype=torch.int32, device=dev), 2 * page, 2 * page, K.F32, out[0], out[1])
+    scale = c.dev["vs"][c.table[0, :2].long().to(dev)].repeat_interleave(page, 0).cpu().double()
+    for got in out.cpu().double():
+        assert ((got - rows.double()).abs().amax(2) <= scale * (0.5 + 127 * 12 * U)).all()
