@@ -276,3 +276,25 @@ def test_no_tile_is_lost(cuda_device, case, kind):
         want, noise = attend_and_noise(q[b:b + 1].double(), k, v, torch.tensor([n]))
         err = (got[b:b + 1].cpu().double() - want).norm(dim=-1)
         assert (err <= norm_bound(want, noise, *roundings(TYPES[kind]))).all(), (b, err)
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-6, 1e6])
+def test_scores_a_step_of_16_apart(cuda_device, size):
+    """Scores around 2^27 log2 units, where f32 has steps of 16: the later keys of each sequence lie one step above the earlier
+    ones, for sequences whose scores have even and odd last digits."""
+    hd, n, first, n_seq = 64, 640, 320, 56
+    lens = [n] * n_seq
+    c = Cache(lens, 16, 1, hd, 25)
+    c.ks[:], c.vs[:] = 1.135e7, size
+    c.k[:] = 0
+    for b in range(n_seq):
+        p = c.table[b].long()
+        c.k[p, 0, :, 0] = 127 - b                # 2^27 .. 2^28 units with the first dim of the query
+        c.k[p[first // 16:], 0, :, 1] = 64       # and 16 more with its second
+        c.v[p[:first // 16]], c.v[p[first // 16:]] = -100, 100
+    c.handle = c.to(cuda_device)
+    q = torch.zeros(n_seq, 1, hd)
+    q[..., 0], q[..., 1] = 1.0, 1.0 / (127 * 65536)  # the smallest step of a query's digits
+    got = run(c, q.to(cuda_device), K.F32, lens, cuda_device).cpu() / size
+    # a score is rounded to half a step, 8 units: the earlier keys together weigh 2^-(16 - 8) of the later at most
+    assert ((got - 100).abs() <= 200 * 2.0 ** -7).all(), got[:, 0, 0]

@@ -23,9 +23,10 @@
 // ticket per pair), adding the parts in CTA order: results do not depend on scheduling.
 //
 // Weights: p = 2^(x - m) with a reference m that moves only when a score passes it by 8 (f32 sum
-// l).  The tensor core takes p vs 2^(m - M) as fp16, where M is the same kind of reference for
+// l).  The tensor core takes p vs 2^-r as fp16, where m + r is the same kind of reference for
 // x + log2 vs: pages whose scales differ by any ratio keep fp16's relative precision against the
-// largest contribution.  For f32 the weights go in as a high and a low fp16 part.
+// largest contribution.  For f32 the weights go in as a high and a low fp16 part.  (r is held by itself and
+// scores are compared by their differences: with m around 2^27 a sum has steps of 16.)
 #include <math.h>
 
 #include <algorithm>
@@ -58,7 +59,7 @@ struct Lay {
     static constexpr int kKBytes = kTile * HD;
     static constexpr int kStage = 2 * kKBytes;
     static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kRecord = 3 * kHeads + kHeads * HD;  // floats: m, l, M, O of one part
+    static constexpr int kRecord = 3 * kHeads + kHeads * HD;  // floats: m, l, r, O of one part
     // the warps' records, later the weights of a block of parts and their references
     static constexpr int kJoinA = kWarps * kRecord * 4, kJoinB = (2 * kBlock * kHeads + kThreads * 2) * 4;
     static constexpr int kJoin = kJoinA > kJoinB ? kJoinA : kJoinB;
@@ -252,6 +253,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
 
     float* rec = reinterpret_cast<float*>(smem + L::kRing);  // the joins' memory
     auto ratio = [](float a, float m) { return a == m ? 1.f : ex2(a - m); };
+    auto join_refs = [](float& m, float& r, float m2, float r2) {  // (NaN, of two that are empty, loses to any number)
+        const float mn = fmaxf(m, m2);
+        r = fmaxf(r + (m - mn), r2 + (m2 - mn));
+        m = mn;
+    };
 
     // ---- a piece: the CTA's part of one pair's tiles
     int n, kvh, h0, nh, mine;  // its tiles; heads; tiles of this warp
@@ -381,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
 #pragma unroll
         for (int j = 0; j < MT; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;             // heads 2 t4 and 2 t4 + 1
-        float r0 = -INFINITY, r1 = -INFINITY, w0 = INFINITY, w1 = INFINITY;  // M, and 2^(m - M)
+        float r0 = -INFINITY, r1 = -INFINITY, w0 = INFINITY, w1 = INFINITY;  // r, and 2^-r
         int slot = 0;
         for (int i = 0; i < mine; i++) {
             if ((i >> 5) != batch) {
@@ -428,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             const float t0 = fmaxf(x0, x2), t1 = fmaxf(x1, x3);
             // (a NaN score never moves a reference; it reaches l and O below)
             float v0 = vs * w0, v1 = vs * w1;  // at most 2^7, so that weights stay below 2^15
-            if (__any_sync(0xffffffffu, t0 > m0 + 8.f || t1 > m1 + 8.f || !(v0 <= 128.f) || !(v1 <= 128.f))) {
+            if (__any_sync(0xffffffffu, t0 - m0 > 8.f || t1 - m1 > 8.f || !(v0 <= 128.f) || !(v1 <= 128.f))) {
                 float c0 = t0, c1 = t1;
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) {
@@ -438,11 +444,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
                 // (log2 of a scale of zero or below the normal range would be -inf, and its weights inf or NaN)
                 const float lv = lg2(fmaxf(vs, 1.17549435e-38f));
                 auto move = [&](float c, float& m, float& l, float& r, float& w, float& v) {
-                    const float mn = fmaxf(m, c), rn = fmaxf(r, c + lv);
-                    l *= m == mn ? 1.f : ex2(m - mn);
-                    const float beta = r == rn ? 1.f : ex2(r - rn);
+                    const float mn = fmaxf(m, c), down = m == mn ? 0.f : m - mn;
+                    const float was = r + down, rn = fmaxf(was, c - mn + lv);
+                    l *= ex2(down);
+                    const float beta = was == rn ? 1.f : ex2(was - rn);
                     m = mn, r = rn;
-                    w = rn == -INFINITY ? INFINITY : ex2(fminf(mn - rn, 127.f));
+                    w = ex2(fminf(-rn, 127.f));
                     v = vs * w;
                     return beta;
                 };
@@ -544,22 +551,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             const int h = i / (HD / 4), d = (i % (HD / 4)) * 4;
             float m = -INFINITY, r = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kWarps; w++) {
-                m = fmaxf(m, rec[w * L::kRecord + h]);
-                r = fmaxf(r, rec[w * L::kRecord + 2 * kHeads + h]);
-            }
+            for (int w = 0; w < kWarps; w++) m = fmaxf(m, rec[w * L::kRecord + h]);
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) r = fmaxf(r, rec[w * L::kRecord + 2 * kHeads + h] + (rec[w * L::kRecord + h] - m));
             float l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < kWarps; w++) {
                 const float* a = rec + w * L::kRecord;
                 if (w >= was_n) break;  // a warp without a tile
                 l += a[kHeads + h] * ratio(a[h], m);
-                const float f = ratio(a[2 * kHeads + h], r);
+                const float f = ratio(a[2 * kHeads + h] + (a[h] - m), r);
                 const float4 v = *reinterpret_cast<const float4*>(a + 3 * kHeads + h * HD + d);
                 y[0] += v.x * f, y[1] += v.y * f, y[2] += v.z * f, y[3] += v.w * f;
             }
             if (whole) {
-                const float f = (r == -INFINITY ? 0.f : ex2(r - m)) / l;
+                const float f = ex2(r) / l;
                 if (h < was_h) store4(out + h * HD + d, y[0] * f, y[1] * f, y[2] * f, y[3] * f);
             } else {
                 if (d == 0) out_rec[h] = m, out_rec[kHeads + h] = l, out_rec[2 * kHeads + h] = r;
@@ -590,18 +596,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
 #pragma unroll 4
                     for (int k = k8; k < parts; k += kRows) {
                         const float* a = part(k);
-                        m = fmaxf(m, __ldcg(a + h8));
-                        r = fmaxf(r, __ldcg(a + 2 * kHeads + h8));
+                        join_refs(m, r, __ldcg(a + h8), __ldcg(a + 2 * kHeads + h8));
                     }
                     ref[k8 * 2 * kHeads + h8] = m;
                     ref[k8 * 2 * kHeads + kHeads + h8] = r;
                 }
                 __syncthreads();
                 float m_all = -INFINITY, r_all = -INFINITY;  // of head h8
-                for (int k = 0; k < kRows; k++) {
-                    m_all = fmaxf(m_all, ref[k * 2 * kHeads + h8]);
-                    r_all = fmaxf(r_all, ref[k * 2 * kHeads + kHeads + h8]);
-                }
+                for (int k = 0; k < kRows; k++)
+                    join_refs(m_all, r_all, ref[k * 2 * kHeads + h8], ref[k * 2 * kHeads + kHeads + h8]);
                 constexpr int kSteps = (kHeads * (HD / 4) + kThreads - 1) / kThreads;
                 float l[kSteps], y[kSteps][4];
 #pragma unroll
@@ -611,8 +614,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
                     __syncthreads();
                     for (int k = k8; k < count; k += kRows) {
                         const float* a = part(k0 + k);
-                        w_l[k * kHeads + h8] = __ldcg(a + kHeads + h8) * ratio(__ldcg(a + h8), m_all);
-                        w_o[k * kHeads + h8] = ratio(__ldcg(a + 2 * kHeads + h8), r_all);
+                        const float m = __ldcg(a + h8);
+                        w_l[k * kHeads + h8] = __ldcg(a + kHeads + h8) * ratio(m, m_all);
+                        w_o[k * kHeads + h8] = ratio(__ldcg(a + 2 * kHeads + h8) + (m - m_all), r_all);
                     }
                     __syncthreads();
 #pragma unroll
@@ -628,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
                         }
                     }
                 }
-                if (k8 == 0) ref[h8] = r_all == -INFINITY ? 0.f : ex2(r_all - m_all);
+                if (k8 == 0) ref[h8] = ex2(r_all);
                 __syncthreads();
 #pragma unroll
                 for (int e = 0; e < kSteps; e++) {
