@@ -16,10 +16,10 @@
 // Bounds, per pair of tiles and 128 keys at head_dim 128: 2048 cycles of exponentials (16 per cycle and
 // SM) and 2350 of the tensor core (S waits for shared memory, 6.5 KB of operands per 40 cycles).  What is
 // reached is 3450: a lone softmax warp's chain of waits, loads, maximum, exponentials and stores.
-// Tried and slower: two threads per lane (519 us for 8192 tokens, 32 heads on 8, against 441), a quarter of the exponentials
+// Tried and slower, at the time: two threads per lane (519 us for 8192 tokens, 32 heads on 8, against 441), a quarter of the exponentials
 // as polynomials (483 against 462), P in the place of S with 128 keys per tile (448), turns of A
 // and B at the exponentials (470).
-// Measured there: 440 us = 1250 TFLOP/s.
+// Measured there: 445 us = 1235 TFLOP/s in single calls, 517 us back to back (the power limit lowers the clock).
 //
 // Softmax: one thread per lane, base 2, with a reference maximum that moves (rescaling O in TMEM and
 // the f32 sum) only when a tile's maximum passes it by 8, so P stays below 2^8.
@@ -45,7 +45,8 @@ constexpr int kTmemCols = 512;
 template <int HD>
 struct Lay {
     static constexpr int BN = HD == 64 ? 128 : HD == 96 ? 96 : 80;  // keys per tile
-    static constexpr int kFirst = HD == 128 ? 80 : 64;  // weights handed over at once, then the rest (measured)
+    // Weights handed over at once, then the rest.  (head_dim 128, 8192 tokens: all 80 at once 441 us, 32, 48 or 64 first 467.)
+    static constexpr int kFirst = HD == 128 ? 80 : 64;
     static constexpr int kP = 2 * BN, kO = 3 * BN;     // TMEM columns: S_A, S_B from 0, P_A, P_B, O_A, O_B
     static constexpr int NC = (HD + 63) / 64;          // 64-column blocks of a row (the last may be part empty)
     static constexpr int kQTile = BM * NC * 128;       // bytes of a tile of Q
@@ -255,7 +256,7 @@ struct alignas(16) Item {
 // The list of items, walked by one warp: the places are ordered by level, then by sequence, where the
 // level is the number of a pair of tiles in its sequence, from the highest down: those with the most keys come first,
 // and nothing is launched for pairs that a short sequence does not have.  (With n_seq x longest indices,
-// 63 prompts of one token beside one of 8192 took 836 us instead of 440.)
+// 63 prompts of one token beside one of 8192 took 836 us instead of 452.)
 constexpr int kSeqs = 2048;  // sequences whose counts are kept in shared memory
 struct List {
     const int* counts;  // [kSeqs]
@@ -616,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float2 y = fma2(make_float2(s[2 * k], s[2 * k + 1]), sc, off);
                         const float2 e = make_float2(ex2(y.x), ex2(y.y));
                         sum[k & 1] = add2(sum[k & 1], e);
-                        x[k] = pack2<T>(e.x, e.y);
+                        x[k] = pack2<T>(e.x, e.y);  // (the product takes 16 bits; the sum takes e, as many roundings average out)
                     }
                 };
                 auto hand_over = [&](int h) {

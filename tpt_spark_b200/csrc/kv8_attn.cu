@@ -40,14 +40,15 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kStages = 3;
-constexpr int kCtasPerSm = 3;  // (4 of 128 registers: 99 us for 8 sequences of 32k against 93)
+constexpr int kCtasPerSm = 3;  // (4, with 128 registers and 2 stages: 98 us for 8 sequences of 32k against 87)
 constexpr int kTile = 16;       // keys
 constexpr int kHeads = 8;       // query heads per pass over the keys (columns of the products)
 constexpr int kBlock = 128;     // parts whose weights are in shared memory at a time
-// Units that make a CTA worth its share of the join (32: 777 positions take 17 us instead of 15, 16384 take 23 instead of 26).
+// Units that make a CTA worth its share of the join (8: 777 positions take 9.8 us instead of 10.4; 32: they take 13.7,
+// and one sequence of 16384 takes 17.6 instead of 18.8; batches that fill the GPU do not notice).
 constexpr int kMinTiles = 16;
 // A pair's place on the line: kSetup units for its queries and its join, then its tiles.  (With tiles alone, ranges
-// of many short sequences took longest: 69 us instead of 56 for 32 sequences of 40 to 8000 positions.)
+// of many short sequences took longest: 74 us instead of 52 for 32 sequences of 40 to 8000 positions; 8 or 32 units: 53.)
 constexpr int kSetup = 16;
 
 template <int HD>
@@ -460,6 +461,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attn_kernel(const __
             const float p0 = ex2(x0 - m0), p1 = ex2(x1 - m1), p2 = ex2(x2 - m0), p3 = ex2(x3 - m1);
             l0 += p0 + p2;
             l1 += p1 + p3;
+            // The product takes 16-bit weights.  fp16, whatever the queries' type: 2^-11 each, below a bf16 output's own
+            // 2^-8; the sum l takes them unrounded, as the roundings of many keys average out.
             uint32_t bh[2], bl[2];
             {
                 const float y0 = p0 * v0, y1 = p1 * v1, y2 = p2 * v0, y3 = p3 * v1;

@@ -42,11 +42,6 @@ __device__ __forceinline__ void unpack8(const Raw8<T>& v, float (&x)[8]) {
             x[2 * i] = __uint_as_float(r[i] << 16), x[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
     }
 }
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-    unpack8<T>(load_raw8(p), x);
-}
-
 // Two f32 as a pair of T in one word (round to nearest), the first in the low half.
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
